@@ -344,6 +344,121 @@ int spork_attn_sm100_fwd_ex(int BH, int S, int D, const void* q, const void* k, 
  * torch_attn.py:40-57): HOST fp32 (N, d) arrays, one head, scale 1/sqrt(d). */
 void htod_f32_attn_sm100_fwd(int N, int d, const float* q, const float* k, const float* v, float* o);
 
+/* ---- Paged key-value cache ------------------------------------------------
+ * What a decoding server needs next to the attention forward: keys and values of
+ * many requests kept in pages of one cache, block tables that say which pages a
+ * request holds, and the attention of one new token per request over them.  The
+ * reference has no counterpart.  Element types of these entry points: */
+#define SPORK_TYPE_F16 0
+#define SPORK_TYPE_BF16 1
+#define SPORK_TYPE_F32 2
+
+/* One cache: k and v hold num_pages pages; element d of row r of head h of page p is
+ * at k[p * k_strides[0] + h * k_strides[1] + r * k_strides[2] + d] (strides in
+ * elements), so either a page's heads ([page][head][row][d]) or its rows
+ * ([page][row][head][d]) may come first in memory.  Token t of a request is row
+ * t % page_size of the page in column t / page_size of its block table; its slot is
+ * page * page_size + row. */
+typedef struct spork_paged_cache {
+    void* k;
+    void* v;
+    int64_t k_strides[3];
+    int64_t v_strides[3];
+    int32_t type; /* SPORK_TYPE_F16 or SPORK_TYPE_BF16 */
+    int32_t num_pages, kv_heads, page_size, head_dim;
+    int32_t reserved;
+} spork_paged_cache;
+
+/* Block tables and slot maps from request lengths.  Request r holds lengths[r]
+ * tokens and is given new_tokens[r] more.  The pages that it lacks for them are taken
+ * from free_pages, in the order of the requests, from entry *free_used on, and
+ * entered into its row of block_table (in place; other entries stay as they are).
+ * A request is refused, i.e. left as it was with no slots for its tokens, if a length
+ * is negative, its table row or the slot map is too short, or the free pages left
+ * by the requests before it (refused for want of pages or not) do not cover its own;
+ * one that needs no page is not refused for want of pages.  Written:
+ *   slots[max_tokens]      the new tokens' slots, request by request; -1 where there
+ *                          is none (a refused request, behind the last token, a
+ *                          negative page)
+ *   offsets[requests + 1]  first token of each request in the slot map, then the total
+ *   lengths_after[requests]
+ *   info[4]                free pages used afterwards, tokens, requests refused, pages
+ *                          asked for (more than were left: the free list ran short)
+ * Sums beyond 2^31 - 1 are written as that.  Inputs and outputs must not overlap.
+ * At most SPORK_PAGED_MAX_REQUESTS requests. */
+#define SPORK_PAGED_MAX_REQUESTS 16384
+typedef struct spork_paged_tables_args {
+    const int32_t* lengths;    /* [requests] */
+    const int32_t* new_tokens; /* [requests] */
+    int32_t* block_table;      /* [requests] rows of max_blocks entries, table_stride apart */
+    const int32_t* free_pages; /* [free_count] */
+    const int32_t* free_used;  /* [1] */
+    int64_t* slots;
+    int32_t* offsets;
+    int32_t* lengths_after;
+    int32_t* info;
+    int64_t table_stride;
+    int64_t max_tokens;
+    int32_t requests, max_blocks, page_size, free_count;
+} spork_paged_tables_args;
+int spork_paged_sm100_tables(const spork_paged_tables_args* args, void* stream);
+
+/* Keys and values of `tokens` tokens into the cache: row t of k and v ([kv_heads][head_dim],
+ * tokens and heads at the given strides, in elements) goes to slots[t], rounded to the
+ * cache's type if it is of another one.  src_type is the cache's type or
+ * SPORK_TYPE_F32 (what the GEMMs write).  A slot outside the cache (-1, say)
+ * writes nothing.  Slots within the cache must differ: of two tokens with the same
+ * one, either's values may remain, piece by piece. */
+typedef struct spork_paged_store_args {
+    spork_paged_cache cache;
+    const void* k;
+    const void* v;
+    const int64_t* slots; /* [tokens] */
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    int64_t tokens;
+    int32_t src_type;
+    int32_t reserved;
+} spork_paged_store_args;
+int spork_paged_sm100_store(const spork_paged_store_args* args, void* stream);
+
+/* Attention of one new token per request over the cache:
+ *   o[r][h] = softmax(scale * q[r][h] . K^T) V over the first lengths[r] keys of
+ *   request r, of key head h / (heads / kv_heads)
+ * q [requests][heads][head_dim] at the given strides (elements), of the cache's type
+ * or fp32; o contiguous, of the cache's type; lse (may be null) [requests][heads]: the
+ * logarithm of the sum of the exponentials, fp32.  A request with no keys gets zeros
+ * and -infinity; one with a negative length, a length beyond its table row or a page
+ * outside the cache among those it needs gets NaN, and nothing outside the cache is
+ * read.  Entries of a table row behind the last page that is needed, and rows of that
+ * page behind the last key, may hold anything.  head_dim 64 or 128; page_size 8, 16,
+ * 32 or a multiple of 64; heads a multiple of kv_heads; k, v and their strides
+ * multiples of 16 bytes; scale positive and finite.
+ * `workspace`: device memory of spork_attn_sm100_paged_workspace bytes, 16-byte
+ * aligned, not read by anything else until the call has run; its contents before
+ * and after do not matter.  Results do not depend on the timing of the run: they are
+ * the same, bit for bit, in every run on the same kind of GPU. */
+typedef struct spork_attn_paged_args {
+    spork_paged_cache cache;
+    const void* q;
+    const int32_t* block_table; /* [requests] rows of max_blocks entries, table_stride apart */
+    const int32_t* lengths;     /* [requests] */
+    void* o;
+    float* lse;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t q_request_stride, q_head_stride;
+    int64_t table_stride;
+    int32_t requests, heads, max_blocks;
+    int32_t q_type;
+    float scale;
+    int32_t reserved;
+} spork_attn_paged_args;
+int spork_attn_sm100_paged_supports(int heads, int kv_heads, int head_dim, int page_size);
+/* Bytes of workspace on the current device; negative: minus an error code. */
+int64_t spork_attn_sm100_paged_workspace(int heads, int kv_heads, int head_dim);
+int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* stream);
+
 /* Library/build information: "spork_b200 <version> sm_100a". */
 const char* spork_b200_version(void);
 

@@ -18,6 +18,9 @@ from .api import (  # noqa: F401
     SEED_B,
     SporkError,
     attn_fwd,
+    attn_paged,
+    attn_paged_supports,
+    attn_paged_workspace,
     choice,
     compare_f32,
     gemm_baseline,
@@ -30,6 +33,8 @@ from .api import (  # noqa: F401
     matmul_sm100_htod,
     matmul_sm100_supports,
     matmul_sm100_tf32,
+    paged_store,
+    paged_tables,
     status,
     ring_model,
     tmap_cache_stats,

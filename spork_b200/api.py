@@ -27,7 +27,7 @@ SEED_B = 19980724
 ERR_BASE = 10000
 _ERR_NAMES = {
     10001: "bad argument (null or misaligned pointer, unknown variant)",
-    10002: "unsupported shape (K must be a multiple of 8)",
+    10002: "unsupported shape (GEMM: K must be a multiple of 8; attention: see the entry point's head dimensions and page sizes)",
     10003: "current device is not an sm_100 (B200-class) GPU",
     10004: "driver call failed (tensor map encode)",
     10005: "a bounded device-side wait ran out",
@@ -116,6 +116,17 @@ def lib() -> ctypes.CDLL:
             L.spork_attn_sm100_fwd_ex.restype = i32
             L.htod_f32_attn_sm100_fwd.argtypes = [i32, i32, vp, vp, vp, vp]
             L.htod_f32_attn_sm100_fwd.restype = None
+        cp = ctypes.c_char_p  # packed argument structures: read before the call returns
+        L.spork_paged_sm100_tables.argtypes = [cp, vp]
+        L.spork_paged_sm100_tables.restype = i32
+        L.spork_paged_sm100_store.argtypes = [cp, vp]
+        L.spork_paged_sm100_store.restype = i32
+        L.spork_attn_sm100_paged.argtypes = [cp, vp]
+        L.spork_attn_sm100_paged.restype = i32
+        L.spork_attn_sm100_paged_supports.argtypes = [i32, i32, i32, i32]
+        L.spork_attn_sm100_paged_supports.restype = i32
+        L.spork_attn_sm100_paged_workspace.argtypes = [i32, i32, i32]
+        L.spork_attn_sm100_paged_workspace.restype = ctypes.c_int64
         L.spork_b200_version.restype = ctypes.c_char_p
         _lib = L
     return _lib
@@ -444,4 +455,260 @@ def attn_fwd(q, k, v, o=None, scale: float | None = None, stream=None, causal: b
                                            _dev_ptr(o, dt, "o"), ctypes.c_float(scale), int(dt == torch.bfloat16),
                                            int(bool(causal)), _stream_ptr(stream))
     _check(rc, "spork_attn_sm100_fwd")
+    return o
+
+
+# --------------------------------------------------------------------------- paged key-value cache
+
+# The argument structures of include/spork_b200.h (spork_paged_cache inside the last two), packed by hand: a call of a
+# few microseconds on the GPU should not wait for ctypes to convert thirty arguments.
+_CACHE = "QQ6q6i"
+_TABLES_ARGS = struct.Struct("=9Q2q4i")
+_STORE_ARGS = struct.Struct("=" + _CACHE + "3Q5q2i")
+_PAGED_ATTN_ARGS = struct.Struct("=" + _CACHE + "6Q4q4ifi")
+_TYPE_CODES = None
+
+
+def _type_code(t, what: str, allowed: str) -> int:
+    global _TYPE_CODES
+    if _TYPE_CODES is None:
+        import torch
+
+        _TYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    code = _TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be {allowed}, got {t.dtype}")
+    return code
+
+
+def _raw_stream(stream, device: int) -> int:
+    """The stream to launch on: the given one, which must be of the tensors' device, or that device's current one."""
+    import torch
+
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device)
+    if stream.device_index != device:
+        raise ValueError(f"the stream is of device {stream.device_index}, the tensors of device {device}")
+    return int(stream.cuda_stream)
+
+
+def _on_gpu(device: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        if t.get_device() != device:
+            raise ValueError(f"tensors are on different devices: {name} on {t.get_device()}, the first on {device}")
+
+
+def _launch(fn, packed: bytes, device: int, stream, what: str) -> None:
+    import torch
+
+    sp = _raw_stream(stream, device)
+    if torch.cuda.current_device() == device:
+        rc = fn(packed, sp)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(packed, sp)
+    if rc:
+        raise SporkError(rc, what)
+
+
+def _new(like, shape, dtype, stream):
+    """An output or scratch tensor that belongs to the stream of the launch."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _vector(t, n, dtype, what: str):
+    """A contiguous 1-D tensor of n elements (any number where n is None)."""
+    if t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{what} must be ({'n' if n is None else n},), got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return t
+
+
+def _block_table(t, requests: int):
+    """(requests, max_blocks) int32, columns contiguous; returns max_blocks and the row stride."""
+    import torch
+
+    if t.dim() != 2 or t.shape[0] != requests:
+        raise ValueError(f"block_table must be ({requests}, max_blocks), got {tuple(t.shape)}")
+    if t.dtype != torch.int32:
+        raise TypeError(f"block_table must be torch.int32, got {t.dtype}")
+    rows, columns = t.stride()
+    if t.shape[1] > 1 and columns != 1:
+        raise ValueError("the entries of a block_table row must be contiguous")
+    return t.shape[1], rows
+
+
+def _pages(k_cache, v_cache):
+    """Shape (num_pages, kv_heads, page_size, head_dim), type code, and strides of a cache's two halves."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError("k_cache and v_cache must both be (num_pages, kv_heads, page_size, head_dim), got "
+                         f"{tuple(shape)} and {tuple(v_cache.shape)}")
+    code = _type_code(k_cache, "k_cache", "float16 or bfloat16")
+    if code == 2 or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"k_cache and v_cache must both be float16 or both bfloat16, got {k_cache.dtype} and {v_cache.dtype}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
+        raise ValueError("the head dimension of a cache must be contiguous")
+    return shape, code, ks[:3], vs[:3]
+
+
+def paged_tables(lengths, new_tokens, block_table, free_pages, free_used, *, page_size: int, max_tokens: int | None = None,
+                 slots=None, offsets=None, lengths_after=None, info=None, stream=None):
+    """Give each request the pages that its new tokens need; returns (slots, offsets, lengths_after, info).
+
+    ``lengths`` and ``new_tokens`` (R,), ``block_table`` (R, max_blocks), ``free_pages`` (F,) and ``free_used`` (1,) are
+    int32 CUDA tensors.  Request r holds ``lengths[r]`` tokens and gets ``new_tokens[r]`` more; the pages that it lacks come
+    from ``free_pages`` in the order of the requests, from entry ``free_used[0]`` on, and are entered into its row of
+    ``block_table`` in place.  ``slots`` (int64) names the place in the cache of every new token, request by request, -1
+    where there is none: it has ``max_tokens`` entries, so that a launch of one size serves steps of any number of tokens.
+    ``offsets`` (R + 1,) says where each request's tokens begin in it.  A request that does not fit (its table row, the
+    slot map, the free list) is left as it was, and ``info`` counts it: [free pages used afterwards, tokens, requests
+    refused, pages asked for].  The rules in full are beside spork_paged_sm100_tables in include/spork_b200.h.  To go on
+    from this step, pass ``lengths_after`` as ``lengths`` and ``info[:1]`` as ``free_used`` (with other outputs: inputs and
+    outputs must not overlap)."""
+    import torch
+
+    i32 = torch.int32
+    if lengths.dim() != 1:
+        raise ValueError(f"lengths must be (R,), got {tuple(lengths.shape)}")
+    n = lengths.shape[0]
+    _vector(lengths, n, i32, "lengths")
+    _vector(new_tokens, n, i32, "new_tokens")
+    _vector(free_pages, None, i32, "free_pages")
+    _vector(free_used, 1, i32, "free_used")
+    blocks, row = _block_table(block_table, n)
+    if not 1 <= page_size < 1 << 31:
+        raise ValueError(f"page_size must be at least 1 and below 2^31, got {page_size}")
+    if slots is None:
+        if max_tokens is None or max_tokens < 0:
+            raise ValueError("max_tokens (or slots) says how many new tokens there is room for")
+        slots = _new(lengths, (max_tokens,), torch.int64, stream)
+    elif max_tokens is not None and slots.shape != (max_tokens,):
+        raise ValueError(f"slots must be ({max_tokens},), got {tuple(slots.shape)}")
+    _vector(slots, None, torch.int64, "slots")
+    offsets = _new(lengths, (n + 1,), i32, stream) if offsets is None else _vector(offsets, n + 1, i32, "offsets")
+    lengths_after = _new(lengths, (n,), i32, stream) if lengths_after is None else _vector(lengths_after, n, i32, "lengths_after")
+    info = _new(lengths, (4,), i32, stream) if info is None else _vector(info, 4, i32, "info")
+    device = lengths.get_device()
+    _on_gpu(device, lengths=lengths, new_tokens=new_tokens, block_table=block_table, free_pages=free_pages,
+            free_used=free_used, slots=slots, offsets=offsets, lengths_after=lengths_after, info=info)
+    packed = _TABLES_ARGS.pack(
+        lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_used.data_ptr(),
+        slots.data_ptr(), offsets.data_ptr(), lengths_after.data_ptr(), info.data_ptr(), row, slots.shape[0], n, blocks,
+        page_size, free_pages.shape[0])
+    _launch(lib().spork_paged_sm100_tables, packed, device, stream, "spork_paged_sm100_tables")
+    return slots, offsets, lengths_after, info
+
+
+def paged_store(k, v, k_cache, v_cache, slots, stream=None):
+    """Write the keys and values of T tokens into their slots of the cache (in place).
+
+    ``k`` and ``v`` are (T, kv_heads, head_dim) with the last dimension contiguous (slices of a projection's rows, say), of
+    the cache's type or float32 (what the GEMMs write; rounded to nearest even).  ``k_cache`` and ``v_cache`` are (num_pages,
+    kv_heads, page_size, head_dim) float16 or bfloat16, the first three dimensions in any order in memory.  ``slots`` (T,)
+    int64 is page * page_size + row, as paged_tables gives it; a slot outside the cache (-1) writes nothing, and slots
+    inside it must differ from each other."""
+    import torch
+
+    shape, code, ks, vs = _pages(k_cache, v_cache)
+    if k.dim() != 3 or k.shape[1] != shape[1] or k.shape[2] != shape[3] or v.shape != k.shape:
+        raise ValueError(f"k and v must both be (T, {shape[1]}, {shape[3]}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    src = _type_code(k, "k", "float32 or the cache's type")
+    if (src != 2 and src != code) or v.dtype != k.dtype:
+        raise TypeError(f"k and v must both be float32 or of the cache's type {k_cache.dtype}, got {k.dtype} and {v.dtype}")
+    kn, vn = k.stride(), v.stride()
+    if shape[3] > 1 and (kn[2] != 1 or vn[2] != 1):
+        raise ValueError("the head dimension of k and v must be contiguous")
+    _vector(slots, k.shape[0], torch.int64, "slots")
+    device = k_cache.get_device()
+    _on_gpu(device, k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots)
+    packed = _STORE_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), *ks, *vs, code, *shape, 0, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
+        kn[0], kn[1], vn[0], vn[1], k.shape[0], src, 0)
+    _launch(lib().spork_paged_sm100_store, packed, device, stream, "spork_paged_sm100_store")
+
+
+def attn_paged_supports(heads: int, kv_heads: int, head_dim: int, page_size: int) -> bool:
+    return bool(lib().spork_attn_sm100_paged_supports(heads, kv_heads, head_dim, page_size))
+
+
+def attn_paged_workspace(heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of workspace that attn_paged needs on the current device, whatever the requests and their lengths."""
+    n = int(lib().spork_attn_sm100_paged_workspace(heads, kv_heads, head_dim))
+    if n < 0:
+        raise SporkError(-n, "spork_attn_sm100_paged_workspace")
+    return n
+
+
+def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, scale: float | None = None, workspace=None,
+               stream=None):
+    """o[r] = softmax(scale q[r] K^T) V over the first ``lengths[r]`` keys that request r holds in the cache.
+
+    One new token per request: ``q`` is (R, heads, head_dim) of the cache's type or float32, with the last dimension
+    contiguous; ``heads`` is a multiple of kv_heads, and query head h reads key head h // (heads // kv_heads).  ``k_cache``
+    and ``v_cache`` are (num_pages, kv_heads, page_size, head_dim), the first three dimensions in any order in memory;
+    ``block_table`` (R, max_blocks) and ``lengths`` (R,) are int32.  ``o`` (contiguous) has the cache's type.  ``lse``, if
+    given, is (R, heads) float32 and receives the logarithm of each softmax's sum.  A request of length 0 gets zeros (lse
+    -inf); one with a length outside its table row or a page outside the cache gets NaN.  ``workspace`` is a contiguous
+    CUDA tensor of attn_paged_workspace bytes, allocated for the call if it is not given; launches that may run at the same
+    time (other streams, other captured graphs) need one each."""
+    import torch
+
+    if q.dim() != 3:
+        raise ValueError(f"q must be (R, heads, head_dim), got {tuple(q.shape)}")
+    n, heads, dim = q.shape
+    shape, code, ks, vs = _pages(k_cache, v_cache)
+    if shape[3] != dim:
+        raise ValueError(f"q has head dimension {dim}, the cache {shape[3]}")
+    q_code = _type_code(q, "q", "float32 or the cache's type")
+    if q_code != 2 and q_code != code:
+        raise TypeError(f"q must be float32 or of the cache's type {k_cache.dtype}, got {q.dtype}")
+    qs = q.stride()
+    if qs[2] != 1:
+        raise ValueError("the head dimension of q must be contiguous")
+    blocks, row = _block_table(block_table, n)
+    _vector(lengths, n, torch.int32, "lengths")
+    if o is None:
+        o = _new(q, (n, heads, dim), k_cache.dtype, stream)
+    elif o.shape != q.shape:
+        raise ValueError(f"o must have q's shape {(n, heads, dim)}, got {tuple(o.shape)}")
+    elif o.dtype != k_cache.dtype:
+        raise TypeError(f"o must be of the cache's type {k_cache.dtype}, got {o.dtype}")
+    elif not o.is_contiguous():
+        raise ValueError("o must be contiguous")
+    if lse is not None:
+        if lse.shape != (n, heads) or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous ({n}, {heads}), got {tuple(lse.shape)}")
+        if lse.dtype != torch.float32:
+            raise TypeError(f"lse must be torch.float32, got {lse.dtype}")
+    device = q.get_device()
+    _on_gpu(device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, o=o)
+    lse_ptr = 0
+    if lse is not None:
+        _on_gpu(device, lse=lse)
+        lse_ptr = lse.data_ptr()
+    if workspace is None:
+        with _OnDevice(device):
+            need = attn_paged_workspace(heads, shape[1], dim)
+        workspace = _new(q, (need,), torch.uint8, stream)
+    else:
+        _on_gpu(device, workspace=workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+    packed = _PAGED_ATTN_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), *ks, *vs, code, *shape, 0, q.data_ptr(), block_table.data_ptr(),
+        lengths.data_ptr(), o.data_ptr(), lse_ptr, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        qs[0], qs[1], row, n, heads, blocks, q_code, 1.0 / dim ** 0.5 if scale is None else scale, 0)
+    _launch(lib().spork_attn_sm100_paged, packed, device, stream, "spork_attn_sm100_paged")
     return o

@@ -1,0 +1,78 @@
+"""Plain implementations of the paged cache's operators for the tests: whole numbers in Python, attention in 64 bits."""
+import math
+
+INT_MAX = 2 ** 31 - 1
+
+
+def tables(lengths, new, table, free, used, page, max_tokens):
+    """The rules of spork_paged_sm100_tables, request by request, on lists (table: list of rows, changed in place)."""
+    left = len(free) - used if 0 <= used <= len(free) else 0
+    slots, offsets, after = [-1] * max_tokens, [], []
+    tokens = pages = granted_pages = refused = 0
+    for r, (held, added) in enumerate(zip(lengths, new)):
+        adds = max(0, added)
+        begin, tokens = tokens, tokens + adds
+        offsets.append(min(begin, INT_MAX))
+        width = len(table[r])
+        sound = held >= 0 and added >= 0 and (adds == 0 or tokens <= max_tokens) and held + adds <= width * page
+        if not sound:
+            refused += 1
+            after.append(held)
+            continue
+        old, total = -(-held // page), -(-(held + adds) // page)
+        base, pages = pages, pages + total - old
+        if total > old and pages > left:
+            refused += 1
+            after.append(held)
+            continue
+        granted_pages += total - old
+        for i in range(total - old):
+            table[r][old + i] = free[used + base + i]
+        for i in range(adds):
+            of = table[r][(held + i) // page]
+            if of >= 0:
+                slots[begin + i] = of * page + (held + i) % page
+        after.append(held + adds)
+    offsets.append(min(tokens, INT_MAX))
+    return slots, offsets, after, [used + granted_pages, min(tokens, INT_MAX), refused, min(pages, INT_MAX)]
+
+
+def attention(q, k, v, scale):
+    """One request: q (heads, D), k and v (kv_heads, keys, D), any type; returns in 64 bits o (heads, D), lse (heads,), and
+    for tolerances the weighted magnitudes sum p |v| (heads, D) and the largest sum |q k| scale of a key (heads,)."""
+    import torch
+
+    heads, dim = q.shape
+    kv_heads, keys, _ = k.shape
+    q, k, v = q.double(), k.double(), v.double()
+    if keys == 0:
+        zero = torch.zeros((heads, dim), dtype=torch.float64, device=q.device)
+        return zero, torch.full((heads,), -math.inf, dtype=torch.float64, device=q.device), zero, zero[:, 0]
+    group = heads // kv_heads
+    kk, vv = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+    x = torch.einsum("hd,hkd->hk", q, kk) * scale
+    size = torch.einsum("hd,hkd->hk", q.abs(), kk.abs()).amax(1) * scale
+    lse = torch.logsumexp(x, 1)
+    p = torch.softmax(x, 1)
+    return (torch.einsum("hk,hkd->hd", p, vv), lse, torch.einsum("hk,hkd->hd", p, vv.abs()), size)
+
+
+def tolerances(dtype, keys, dim, ref, weighted, size, fp32_q):
+    """How far o and lse may be from the 64-bit values.
+
+    Scores: dim products of 16-bit factors are exact in 32 bits, their sum is off by at most dim steps of 2^-23 (the tensor
+    core may truncate) of the sum of their magnitudes; a 32-bit q is taken as two 16-bit parts, which leaves (eps / 2)^2 of
+    it (for fp16 at least 2^-25 absolutely, a subnormal's half step, on q of a size around one: within the same bound
+    times four); scaling, subtracting the maximum and the exponential add a few 2^-23 of the score's magnitude.  A score off by e moves a weight
+    by e and, through the sum, the others by e: 2 e of the weighted magnitudes.  Weights: taken as two 16-bit parts of
+    numbers up to 2^8, (eps / 2)^2, and a key whose weight is below the smallest step (2^-33 of the largest) by that much.
+    Sums over the keys: at most one step of 2^-23 for every key and joining, of the weighted magnitudes.  At the end o is
+    rounded once: eps / 2 of its own value (below the normal range: half the smallest step)."""
+    import torch
+
+    half = torch.finfo(dtype).eps / 2
+    e = size * ((dim + 8) * 2.0 ** -23 + (4 * half * half if fp32_q else 0.0)) + 2.0 ** -21
+    inner = 2 * e + half * half + keys * 2.0 ** -33 + (keys + 64) * 2.0 ** -23
+    tol_o = half * ref.abs() + (1 + half) * inner[:, None] * weighted + torch.finfo(dtype).smallest_normal * half
+    tol_lse = e + (keys + 64) * 2.0 ** -23 + 2.0 ** -23 * (size + math.log(max(keys, 1)) + 1)
+    return tol_o, tol_lse
