@@ -374,7 +374,7 @@ typedef struct spork_paged_cache {
  * from free_pages, in the order of the requests, from entry *free_used on, and
  * entered into its row of block_table (in place; other entries stay as they are).
  * A request is refused, i.e. left as it was with no slots for its tokens, if a length
- * is negative, its table row or the slot map is too short, or the free pages left
+ * is negative, its table row (or 2^31 - 1 tokens) or the slot map is too short, or the free pages left
  * by the requests before it (refused for want of pages or not) do not cover its own;
  * one that needs no page is not refused for want of pages.  Written:
  *   slots[max_tokens]      the new tokens' slots, request by request; -1 where there

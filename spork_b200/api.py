@@ -466,48 +466,48 @@ _CACHE = "QQ6q6i"
 _TABLES_ARGS = struct.Struct("=9Q2q4i")
 _STORE_ARGS = struct.Struct("=" + _CACHE + "3Q5q2i")
 _PAGED_ATTN_ARGS = struct.Struct("=" + _CACHE + "6Q4q4ifi")
-_TYPE_CODES = None
+# torch, its types' codes and its unwrapped calls, once a call below has needed them: these functions stand in front of
+# kernels of a few microseconds, so they look each property of a tensor up once and call as little as they can
+_T = None
+_TYPE_CODES: dict = {}
+_current_device = _raw_stream = None
+_workspace_bytes: dict = {}
 
 
-def _type_code(t, what: str, allowed: str) -> int:
-    global _TYPE_CODES
-    if _TYPE_CODES is None:
-        import torch
-
-        _TYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-    code = _TYPE_CODES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what} must be {allowed}, got {t.dtype}")
-    return code
-
-
-def _raw_stream(stream, device: int) -> int:
-    """The stream to launch on: the given one, which must be of the tensors' device, or that device's current one."""
+def _bind_torch():
+    global _T, _current_device, _raw_stream
     import torch
 
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(device)
-    if stream.device_index != device:
-        raise ValueError(f"the stream is of device {stream.device_index}, the tensors of device {device}")
-    return int(stream.cuda_stream)
+    _TYPE_CODES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _T = torch
+    return torch
 
 
-def _on_gpu(device: int, **tensors) -> None:
+def _on_gpu(**tensors) -> None:
+    """Raise for the tensor that is not where the first one is, on one GPU."""
+    device = None
     for name, t in tensors.items():
         if not t.is_cuda:
             raise TypeError(f"{name} must be a CUDA tensor")
+        if device is None:
+            first, device = name, t.get_device()
         if t.get_device() != device:
-            raise ValueError(f"tensors are on different devices: {name} on {t.get_device()}, the first on {device}")
+            raise ValueError(f"tensors are on different devices: {first} on {device}, {name} on {t.get_device()}")
 
 
 def _launch(fn, packed: bytes, device: int, stream, what: str) -> None:
-    import torch
-
-    sp = _raw_stream(stream, device)
-    if torch.cuda.current_device() == device:
+    """Launch on the given stream, which must be of the tensors' device, or on that device's current one."""
+    if stream is None:
+        sp = _raw_stream(device)
+    elif stream.device_index != device:
+        raise ValueError(f"the stream is of device {stream.device_index}, the tensors of device {device}")
+    else:
+        sp = stream.cuda_stream
+    if _current_device() == device:
         rc = fn(packed, sp)
     else:
-        with torch.cuda.device(device):
+        with _T.cuda.device(device):
             rc = fn(packed, sp)
     if rc:
         raise SporkError(rc, what)
@@ -515,19 +515,18 @@ def _launch(fn, packed: bytes, device: int, stream, what: str) -> None:
 
 def _new(like, shape, dtype, stream):
     """An output or scratch tensor that belongs to the stream of the launch."""
-    import torch
-
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return _T.empty(shape, dtype=dtype, device=like.device)
+    with _T.cuda.stream(stream):
+        return _T.empty(shape, dtype=dtype, device=like.device)
 
 
 def _vector(t, n, dtype, what: str):
-    """A contiguous 1-D tensor of n elements (any number where n is None)."""
-    if t.dim() != 1 or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{what} must be ({'n' if n is None else n},), got {tuple(t.shape)}")
-    if t.dtype != dtype:
+    """Raise unless t is a contiguous 1-D tensor of n elements (any number where n is None)."""
+    shape = t.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n):
+        raise ValueError(f"{what} must be ({'n' if n is None else n},), got {tuple(shape)}")
+    if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
@@ -536,31 +535,30 @@ def _vector(t, n, dtype, what: str):
 
 def _block_table(t, requests: int):
     """(requests, max_blocks) int32, columns contiguous; returns max_blocks and the row stride."""
-    import torch
-
-    if t.dim() != 2 or t.shape[0] != requests:
-        raise ValueError(f"block_table must be ({requests}, max_blocks), got {tuple(t.shape)}")
-    if t.dtype != torch.int32:
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != requests:
+        raise ValueError(f"block_table must be ({requests}, max_blocks), got {tuple(shape)}")
+    if t.dtype is not _T.int32:
         raise TypeError(f"block_table must be torch.int32, got {t.dtype}")
     rows, columns = t.stride()
-    if t.shape[1] > 1 and columns != 1:
+    if columns != 1 and shape[1] > 1:
         raise ValueError("the entries of a block_table row must be contiguous")
-    return t.shape[1], rows
+    return shape[1], rows
 
 
 def _pages(k_cache, v_cache):
     """Shape (num_pages, kv_heads, page_size, head_dim), type code, and strides of a cache's two halves."""
-    shape = k_cache.shape
+    shape, dtype = k_cache.shape, k_cache.dtype
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must both be (num_pages, kv_heads, page_size, head_dim), got "
                          f"{tuple(shape)} and {tuple(v_cache.shape)}")
-    code = _type_code(k_cache, "k_cache", "float16 or bfloat16")
-    if code == 2 or v_cache.dtype != k_cache.dtype:
-        raise TypeError(f"k_cache and v_cache must both be float16 or both bfloat16, got {k_cache.dtype} and {v_cache.dtype}")
+    code = _TYPE_CODES.get(dtype, 2)
+    if code == 2 or v_cache.dtype is not dtype:
+        raise TypeError(f"k_cache and v_cache must both be float16 or both bfloat16, got {dtype} and {v_cache.dtype}")
     ks, vs = k_cache.stride(), v_cache.stride()
-    if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
+    if (ks[3] != 1 or vs[3] != 1) and shape[3] > 1:
         raise ValueError("the head dimension of a cache must be contiguous")
-    return shape, code, ks[:3], vs[:3]
+    return shape, code, ks, vs
 
 
 def paged_tables(lengths, new_tokens, block_table, free_pages, free_used, *, page_size: int, max_tokens: int | None = None,
@@ -577,12 +575,12 @@ def paged_tables(lengths, new_tokens, block_table, free_pages, free_used, *, pag
     refused, pages asked for].  The rules in full are beside spork_paged_sm100_tables in include/spork_b200.h.  To go on
     from this step, pass ``lengths_after`` as ``lengths`` and ``info[:1]`` as ``free_used`` (with other outputs: inputs and
     outputs must not overlap)."""
-    import torch
-
+    torch = _T or _bind_torch()
     i32 = torch.int32
-    if lengths.dim() != 1:
-        raise ValueError(f"lengths must be (R,), got {tuple(lengths.shape)}")
-    n = lengths.shape[0]
+    shape = lengths.shape
+    if len(shape) != 1:
+        raise ValueError(f"lengths must be (R,), got {tuple(shape)}")
+    n = shape[0]
     _vector(lengths, n, i32, "lengths")
     _vector(new_tokens, n, i32, "new_tokens")
     _vector(free_pages, None, i32, "free_pages")
@@ -594,20 +592,22 @@ def paged_tables(lengths, new_tokens, block_table, free_pages, free_used, *, pag
         if max_tokens is None or max_tokens < 0:
             raise ValueError("max_tokens (or slots) says how many new tokens there is room for")
         slots = _new(lengths, (max_tokens,), torch.int64, stream)
-    elif max_tokens is not None and slots.shape != (max_tokens,):
-        raise ValueError(f"slots must be ({max_tokens},), got {tuple(slots.shape)}")
-    _vector(slots, None, torch.int64, "slots")
+    else:
+        _vector(slots, max_tokens, torch.int64, "slots")
     offsets = _new(lengths, (n + 1,), i32, stream) if offsets is None else _vector(offsets, n + 1, i32, "offsets")
     lengths_after = _new(lengths, (n,), i32, stream) if lengths_after is None else _vector(lengths_after, n, i32, "lengths_after")
     info = _new(lengths, (4,), i32, stream) if info is None else _vector(info, 4, i32, "info")
     device = lengths.get_device()
-    _on_gpu(device, lengths=lengths, new_tokens=new_tokens, block_table=block_table, free_pages=free_pages,
-            free_used=free_used, slots=slots, offsets=offsets, lengths_after=lengths_after, info=info)
+    if device < 0 or not (device == new_tokens.get_device() == block_table.get_device() == free_pages.get_device()
+                          == free_used.get_device() == slots.get_device() == offsets.get_device()
+                          == lengths_after.get_device() == info.get_device()):
+        _on_gpu(lengths=lengths, new_tokens=new_tokens, block_table=block_table, free_pages=free_pages,
+                free_used=free_used, slots=slots, offsets=offsets, lengths_after=lengths_after, info=info)
     packed = _TABLES_ARGS.pack(
         lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_used.data_ptr(),
         slots.data_ptr(), offsets.data_ptr(), lengths_after.data_ptr(), info.data_ptr(), row, slots.shape[0], n, blocks,
         page_size, free_pages.shape[0])
-    _launch(lib().spork_paged_sm100_tables, packed, device, stream, "spork_paged_sm100_tables")
+    _launch((_lib or lib()).spork_paged_sm100_tables, packed, device, stream, "spork_paged_sm100_tables")
     return slots, offsets, lengths_after, info
 
 
@@ -619,24 +619,26 @@ def paged_store(k, v, k_cache, v_cache, slots, stream=None):
     kv_heads, page_size, head_dim) float16 or bfloat16, the first three dimensions in any order in memory.  ``slots`` (T,)
     int64 is page * page_size + row, as paged_tables gives it; a slot outside the cache (-1) writes nothing, and slots
     inside it must differ from each other."""
-    import torch
-
+    torch = _T or _bind_torch()
     shape, code, ks, vs = _pages(k_cache, v_cache)
-    if k.dim() != 3 or k.shape[1] != shape[1] or k.shape[2] != shape[3] or v.shape != k.shape:
-        raise ValueError(f"k and v must both be (T, {shape[1]}, {shape[3]}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    src = _type_code(k, "k", "float32 or the cache's type")
-    if (src != 2 and src != code) or v.dtype != k.dtype:
+    pages, kv_heads, page, dim = shape
+    tokens = k.shape
+    if v.shape != tokens or len(tokens) != 3 or tokens[1] != kv_heads or tokens[2] != dim:
+        raise ValueError(f"k and v must both be (T, {kv_heads}, {dim}), got {tuple(tokens)} and {tuple(v.shape)}")
+    src = _TYPE_CODES.get(k.dtype)
+    if (src != 2 and src != code) or v.dtype is not k.dtype:
         raise TypeError(f"k and v must both be float32 or of the cache's type {k_cache.dtype}, got {k.dtype} and {v.dtype}")
     kn, vn = k.stride(), v.stride()
-    if shape[3] > 1 and (kn[2] != 1 or vn[2] != 1):
+    if (kn[2] != 1 or vn[2] != 1) and dim > 1:
         raise ValueError("the head dimension of k and v must be contiguous")
-    _vector(slots, k.shape[0], torch.int64, "slots")
+    _vector(slots, tokens[0], torch.int64, "slots")
     device = k_cache.get_device()
-    _on_gpu(device, k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots)
+    if device < 0 or not (device == v_cache.get_device() == k.get_device() == v.get_device() == slots.get_device()):
+        _on_gpu(k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots)
     packed = _STORE_ARGS.pack(
-        k_cache.data_ptr(), v_cache.data_ptr(), *ks, *vs, code, *shape, 0, k.data_ptr(), v.data_ptr(), slots.data_ptr(),
-        kn[0], kn[1], vn[0], vn[1], k.shape[0], src, 0)
-    _launch(lib().spork_paged_sm100_store, packed, device, stream, "spork_paged_sm100_store")
+        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], code, pages, kv_heads, page, dim, 0,
+        k.data_ptr(), v.data_ptr(), slots.data_ptr(), kn[0], kn[1], vn[0], vn[1], tokens[0], src, 0)
+    _launch((_lib or lib()).spork_paged_sm100_store, packed, device, stream, "spork_paged_sm100_store")
 
 
 def attn_paged_supports(heads: int, kv_heads: int, head_dim: int, page_size: int) -> bool:
@@ -663,52 +665,59 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     -inf); one with a length outside its table row or a page outside the cache gets NaN.  ``workspace`` is a contiguous
     CUDA tensor of attn_paged_workspace bytes, allocated for the call if it is not given; launches that may run at the same
     time (other streams, other captured graphs) need one each."""
-    import torch
-
-    if q.dim() != 3:
-        raise ValueError(f"q must be (R, heads, head_dim), got {tuple(q.shape)}")
-    n, heads, dim = q.shape
+    torch = _T or _bind_torch()
+    q_shape = q.shape
+    if len(q_shape) != 3:
+        raise ValueError(f"q must be (R, heads, head_dim), got {tuple(q_shape)}")
+    n, heads, dim = q_shape
     shape, code, ks, vs = _pages(k_cache, v_cache)
-    if shape[3] != dim:
-        raise ValueError(f"q has head dimension {dim}, the cache {shape[3]}")
-    q_code = _type_code(q, "q", "float32 or the cache's type")
+    pages, kv_heads, page, cache_dim = shape
+    if cache_dim != dim:
+        raise ValueError(f"q has head dimension {dim}, the cache {cache_dim}")
+    dtype = k_cache.dtype
+    q_code = _TYPE_CODES.get(q.dtype)
     if q_code != 2 and q_code != code:
-        raise TypeError(f"q must be float32 or of the cache's type {k_cache.dtype}, got {q.dtype}")
+        raise TypeError(f"q must be float32 or of the cache's type {dtype}, got {q.dtype}")
     qs = q.stride()
     if qs[2] != 1:
         raise ValueError("the head dimension of q must be contiguous")
     blocks, row = _block_table(block_table, n)
     _vector(lengths, n, torch.int32, "lengths")
     if o is None:
-        o = _new(q, (n, heads, dim), k_cache.dtype, stream)
-    elif o.shape != q.shape:
+        o = _new(q, (n, heads, dim), dtype, stream)
+    elif o.shape != q_shape:
         raise ValueError(f"o must have q's shape {(n, heads, dim)}, got {tuple(o.shape)}")
-    elif o.dtype != k_cache.dtype:
-        raise TypeError(f"o must be of the cache's type {k_cache.dtype}, got {o.dtype}")
+    elif o.dtype is not dtype:
+        raise TypeError(f"o must be of the cache's type {dtype}, got {o.dtype}")
     elif not o.is_contiguous():
         raise ValueError("o must be contiguous")
     if lse is not None:
         if lse.shape != (n, heads) or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous ({n}, {heads}), got {tuple(lse.shape)}")
-        if lse.dtype != torch.float32:
+        if lse.dtype is not torch.float32:
             raise TypeError(f"lse must be torch.float32, got {lse.dtype}")
     device = q.get_device()
-    _on_gpu(device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, o=o)
-    lse_ptr = 0
-    if lse is not None:
-        _on_gpu(device, lse=lse)
-        lse_ptr = lse.data_ptr()
+    if device < 0 or not (device == k_cache.get_device() == v_cache.get_device() == block_table.get_device()
+                          == lengths.get_device() == o.get_device()) or (lse is not None and lse.get_device() != device):
+        _on_gpu(q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, o=o,
+                **({} if lse is None else {"lse": lse}))
     if workspace is None:
-        with _OnDevice(device):
-            need = attn_paged_workspace(heads, shape[1], dim)
+        key = (device, heads, kv_heads, dim)
+        need = _workspace_bytes.get(key)
+        if need is None:
+            with _OnDevice(device):
+                need = _workspace_bytes[key] = attn_paged_workspace(heads, kv_heads, dim)
         workspace = _new(q, (need,), torch.uint8, stream)
     else:
-        _on_gpu(device, workspace=workspace)
+        need = workspace.numel() * workspace.element_size()
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
+        if workspace.get_device() != device:
+            _on_gpu(q=q, workspace=workspace)
     packed = _PAGED_ATTN_ARGS.pack(
-        k_cache.data_ptr(), v_cache.data_ptr(), *ks, *vs, code, *shape, 0, q.data_ptr(), block_table.data_ptr(),
-        lengths.data_ptr(), o.data_ptr(), lse_ptr, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        qs[0], qs[1], row, n, heads, blocks, q_code, 1.0 / dim ** 0.5 if scale is None else scale, 0)
-    _launch(lib().spork_attn_sm100_paged, packed, device, stream, "spork_attn_sm100_paged")
+        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], code, pages, kv_heads, page, dim, 0,
+        q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        workspace.data_ptr(), need, qs[0], qs[1], row, n, heads, blocks, q_code,
+        1.0 / dim ** 0.5 if scale is None else scale, 0)
+    _launch((_lib or lib()).spork_attn_sm100_paged, packed, device, stream, "spork_attn_sm100_paged")
     return o

@@ -4,34 +4,48 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <mutex>
 #include <stdint.h>
 
 #include "../../include/spork_b200.h"
 #include "device_state.h"
 #include "paged_sm100.h"
+#include "ptx_sm100.cuh"
 
 namespace spork {
 namespace paged_sm100 {
 
-constexpr int kTableThreads = 1024;
+using namespace spork::ptx;
+
+// ------------------------------------------------------------------ block tables and slot maps
+//
+// Two sums over the requests say where each one's tokens lie in the slot map and which of the free pages it gets.  The
+// list is short (it is one entry per request) and everything else depends on it, so every block takes both sums over all
+// requests for itself, keeps them in shared memory, and then fills its share of the slot map and of the new table
+// entries, finding the request of a token or page by bisection: one launch, and blocks that do not wait for one another.
+// A decoding step is bound by the latency of one dependent chain (lengths, sums, page, slot); a queue of prompts by
+// writing the slot map.
+
+constexpr int kTableThreads = 512;
 
 __device__ __forceinline__ int32_t saturate(int64_t v) { return v > 0x7FFFFFFF ? 0x7FFFFFFF : (int32_t)v; }
 
-// Inclusive sum over the block; `total` receives the block's.
-__device__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t& total)
+// Inclusive sum over the block's threads; `total` receives the block's.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t& total)
 {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const int64_t w = __shfl_up_sync(0xFFFFFFFFu, v, d);
         v += lane >= d ? w : 0;
     }
-    __syncthreads();
     if (lane == 31) {
         warp_sums[warp] = v;
     }
     __syncthreads();
     total = 0;
     int64_t before = 0;
+#pragma unroll
     for (int w = 0; w < kTableThreads / 32; ++w) {
         before += w < warp ? warp_sums[w] : 0;
         total += warp_sums[w];
@@ -39,84 +53,289 @@ __device__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t& total)
     return before + v;
 }
 
-// One block; a thread per request, blocks of requests one after the other.
+// What a thread knows of one of its requests, given the tokens of all before it.
+struct Request {
+    int64_t held, adds, need;
+    bool sound;
+    __device__ __forceinline__ Request(const spork_paged_tables_args& a, int r, int64_t tokens_before)
+    {
+        held = a.lengths[r];
+        const int64_t added = a.new_tokens[r];
+        adds = added > 0 ? added : 0;
+        sound = held >= 0 && added >= 0 && (adds == 0 || tokens_before + adds <= a.max_tokens) &&
+                held + adds <= (int64_t)a.max_blocks * a.page_size && held + adds <= 0x7FFFFFFF;
+        need = sound ? (int64_t)pages_of(held + adds, a.page_size) - (int64_t)pages_of(held, a.page_size) : 0;
+    }
+    // of 0 .. 2^31 - 1 tokens
+    static __device__ __forceinline__ uint32_t pages_of(int64_t tokens, uint32_t page)
+    {
+        return ((uint32_t)tokens + page - 1u) / page;
+    }
+};
+
+// Last of the n ascending entries that is at most v (the first one is).
+__device__ __forceinline__ int last_at_most(const int32_t* entries, int n, int32_t v)
+{
+    int low = 0;
+    while (n > 1) {
+        const int half = n / 2;
+        const bool up = entries[low + half] <= v;
+        low = up ? low + half : low;
+        n = up ? n - half : half;
+    }
+    return low;
+}
+
 __global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged_tables_args a)
 {
-    __shared__ int64_t warp_sums[kTableThreads / 32];
-    const int64_t page = a.page_size, capacity = (int64_t)a.max_blocks * page;
-    const int64_t used = *a.free_used;
+    // per request: first token in the slot map, first page among the granted ones, tokens held (-1: refused)
+    extern __shared__ int32_t per_request[];
+    __shared__ int64_t token_sums[kTableThreads / 32], page_sums[kTableThreads / 32];
+    __shared__ int granted_pages, refused;
+    const int n = a.requests;
+    int32_t *first_token = per_request, *first_page = per_request + n, *held_of = per_request + 2 * n;
+    if (threadIdx.x == 0) {
+        granted_pages = refused = 0;
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int32_t used = *a.free_used;
     const int64_t left = used >= 0 && used <= a.free_count ? a.free_count - used : 0;
-    int64_t tokens = 0, pages = 0, granted_pages = 0, refused = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += kTableThreads) {
-        const int r = r0 + (int)threadIdx.x;
-        const bool mine = r < a.requests;
-        const int64_t held = mine ? a.lengths[r] : 0, added = mine ? a.new_tokens[r] : 0;
-        const int64_t adds = added > 0 ? added : 0;
-        int64_t total;
-        const int64_t ends = tokens + block_scan(adds, warp_sums, total);
-        tokens += total;
-        const bool sound = held >= 0 && added >= 0 && (adds == 0 || ends <= a.max_tokens) && held + adds <= capacity;
-        const int64_t old = sound ? (held + page - 1) / page : 0;
-        const int64_t need = sound ? (held + adds + page - 1) / page - old : 0;
-        const int64_t until = pages + block_scan(need, warp_sums, total);
-        pages += total;
-        const bool granted = sound && (need == 0 || until <= left);
-        block_scan(granted ? need : 0, warp_sums, total);
-        granted_pages += total;
-        block_scan(granted || !mine ? 0 : 1, warp_sums, total);
-        refused += total;
-        if (mine) {
-            const int32_t* from = a.free_pages + used + (until - need);
-            int32_t* row = a.block_table + r * a.table_stride;
-            a.offsets[r] = saturate(ends - adds);
-            a.lengths_after[r] = granted ? (int32_t)(held + adds) : (int32_t)held;
-            for (int64_t i = 0; i < need && granted; ++i) {
-                row[old + i] = from[i];
+    const int chunk = (n + kTableThreads - 1) / kTableThreads;
+    const int r0 = (int)threadIdx.x * chunk < n ? (int)threadIdx.x * chunk : n, r1 = r0 + chunk < n ? r0 + chunk : n;
+
+    int64_t mine = 0, tokens, pages;
+    for (int r = r0; r < r1; ++r) {
+        const int32_t added = a.new_tokens[r];
+        mine += added > 0 ? added : 0;
+    }
+    const int64_t token0 = block_scan(mine, token_sums, tokens) - mine;
+    int64_t token = token0;
+    mine = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Request q(a, r, token);
+        token += q.adds;
+        mine += q.need;
+    }
+    int64_t page = block_scan(mine, page_sums, pages) - mine;
+    token = token0;
+    int most = 0, not_granted = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Request q(a, r, token);
+        const bool granted = q.sound && (q.need == 0 || page + q.need <= left);
+        first_token[r] = saturate(token);
+        first_page[r] = saturate(page);
+        held_of[r] = granted ? (int32_t)q.held : -1;
+        if (blockIdx.x == 0) {
+            a.offsets[r] = saturate(token);
+            a.lengths_after[r] = (int32_t)(granted ? q.held + q.adds : q.held);
+        }
+        token += q.adds;
+        page += q.need;
+        // what is granted ends where the last granted request with pages does
+        most = granted && q.need > 0 ? (int)page : most;
+        not_granted += granted ? 0 : 1;
+    }
+    if (most > 0) {
+        atomicMax(&granted_pages, most);
+    }
+    if (not_granted > 0) {
+        atomicAdd(&refused, not_granted);
+    }
+    __syncthreads();
+
+    const int granted = granted_pages;
+    const int stride = gridDim.x * kTableThreads, at = blockIdx.x * kTableThreads + threadIdx.x;
+    if (at == 0) {
+        a.offsets[n] = saturate(tokens);
+        a.info[0] = saturate((int64_t)used + granted);
+        a.info[1] = saturate(tokens);
+        a.info[2] = refused;
+        a.info[3] = saturate(pages);
+    }
+    const uint32_t page_size = a.page_size;
+    for (int i = at; i < granted; i += stride) {
+        const int r = last_at_most(first_page, n, i);
+        const uint32_t old = Request::pages_of(held_of[r], page_size);
+        a.block_table[r * a.table_stride + old + (i - first_page[r])] = a.free_pages[used + i];
+    }
+    for (int64_t t = at; t < a.max_tokens; t += stride) {
+        int64_t slot = -1;
+        if (t < tokens) {
+            const int r = last_at_most(first_token, n, (int32_t)t);
+            const int32_t held = held_of[r];
+            if (held >= 0) {
+                const uint32_t place = (uint32_t)held + (uint32_t)(t - first_token[r]);
+                const uint32_t block = place / page_size, old = Request::pages_of(held, page_size);
+                const int32_t of = block < old ? a.block_table[r * a.table_stride + block]
+                                               : a.free_pages[used + first_page[r] + (int)(block - old)];
+                slot = of >= 0 ? (int64_t)of * page_size + (place - block * page_size) : -1;
             }
-            for (int64_t i = 0; i < adds && ends - adds + i < a.max_tokens; ++i) {
-                const int64_t at = held + i;
-                const int64_t of = granted ? row[at / page] : -1;
-                a.slots[ends - adds + i] = of >= 0 ? of * page + at % page : -1;
+        }
+        a.slots[t] = slot;
+    }
+}
+
+// ------------------------------------------------------------------ keys and values into their slots
+//
+// Bound by HBM: every element is read once and written once, 16 bytes of the cache at a time where pointers and strides
+// allow it.  A thread keeps its place in a token's row (which half, head, column) and takes it for kTokens tokens, whose
+// slots and elements it asks for before it needs the first one.
+
+constexpr int kStoreThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void load_elements(const T* p, T (&x)[1]) { x[0] = *p; }
+template <typename T>
+__device__ __forceinline__ void load_elements(const T* p, T (&x)[8])
+{
+    const uint4* from = reinterpret_cast<const uint4*>(p);
+    uint4* to = reinterpret_cast<uint4*>(x);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        to[i] = __ldg(from + i);
+    }
+}
+
+template <typename Dst, typename Src>
+__device__ __forceinline__ void store_elements(Dst* p, const Src (&x)[1]) { *p = round_to<Dst>(x[0]); }
+template <typename Dst, typename Src>
+__device__ __forceinline__ void store_elements(Dst* p, const Src (&x)[8])
+{
+    uint4 v;
+    Dst* y = reinterpret_cast<Dst*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = round_to<Dst>(x[i]);
+    }
+    *reinterpret_cast<uint4*>(p) = v;
+}
+
+struct StoreShape {
+    int items, per_head;  // pieces of a token's keys and values together, and of one head
+    int rows;             // tokens that a block takes side by side
+};
+
+template <typename Src, typename Dst, int kElems, int kTokens>
+__global__ void __launch_bounds__(kStoreThreads) store_kernel(const spork_paged_store_args a, const StoreShape shape)
+{
+    static_assert(kElems == 8 || kElems == 1, "16 bytes of the cache, or one element");
+    const spork_paged_cache& c = a.cache;
+    const int64_t slots = (int64_t)c.num_pages * c.page_size;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    for (int i = threadIdx.x; i < shape.items * shape.rows; i += kStoreThreads) {
+        const int row = i / shape.items, half = shape.items / 2;
+        int item = i - row * shape.items;
+        const bool value = item >= half;
+        item -= value ? half : 0;
+        const int h = item / shape.per_head, d = (item - h * shape.per_head) * kElems;
+        const int64_t token_stride = value ? a.v_token_stride : a.k_token_stride;
+        const Src* src = static_cast<const Src*>(value ? a.v : a.k) + h * (value ? a.v_head_stride : a.k_head_stride) + d;
+        const int64_t* strides = value ? c.v_strides : c.k_strides;
+        const int64_t page_stride = strides[0], row_stride = strides[2];
+        Dst* dst = static_cast<Dst*>(value ? c.v : c.k) + h * strides[1] + d;
+        const int64_t t0 = (int64_t)blockIdx.x * (shape.rows * kTokens) + row;
+        int64_t slot[kTokens];
+        alignas(16) Src x[kTokens][kElems];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+            const int64_t t = t0 + j * shape.rows;
+            slot[j] = t < a.tokens ? a.slots[t] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+            const int64_t t = t0 + j * shape.rows;
+            if (t < a.tokens) {
+                load_elements(src + t * token_stride, x[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+            if (slot[j] >= 0 && slot[j] < slots) {
+                const int64_t page = slots <= 0x7FFFFFFF ? (uint32_t)slot[j] / (uint32_t)c.page_size : slot[j] / c.page_size;
+                store_elements(dst + page * page_stride + (slot[j] - page * c.page_size) * row_stride, x[j]);
             }
         }
     }
-    for (int64_t t = tokens + threadIdx.x; t < a.max_tokens; t += kTableThreads) {
-        a.slots[t] = -1;
-    }
-    if (threadIdx.x == 0) {
-        a.offsets[a.requests] = saturate(tokens);
-        a.info[0] = saturate(used + granted_pages);
-        a.info[1] = saturate(tokens);
-        a.info[2] = (int32_t)refused;
-        a.info[3] = saturate(pages);
-    }
 }
 
-// One block per token.
-template <typename Src, typename Dst>
-__global__ void store_kernel(const spork_paged_store_args a)
+// A launch that may begin while the kernel before it in the stream is finishing (the kernels wait for it themselves).
+template <typename... Params, typename... Args>
+static int launch(void (*kernel)(Params...), unsigned blocks, int threads, size_t smem, cudaStream_t stream, const Args&... args)
 {
-    const int64_t t = blockIdx.x;
-    const int64_t slot = a.slots[t];
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+static int launch_tables(const spork_paged_tables_args& a, DeviceState& dev, cudaStream_t stream)
+{
+    const size_t smem = (size_t)a.requests * 3 * sizeof(int32_t);
+    if (smem > 40 * 1024) {  // beyond what a kernel gets unasked (its static arrays included)
+        static std::once_flag once[kMaxDevices];
+        static cudaError_t err[kMaxDevices];
+        std::call_once(once[dev.ordinal], [&] {
+            err[dev.ordinal] = cudaFuncSetAttribute(tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                    SPORK_PAGED_MAX_REQUESTS * 3 * (int)sizeof(int32_t));
+        });
+        if (err[dev.ordinal] != cudaSuccess) {
+            return (int)err[dev.ordinal];
+        }
+    }
+    const int64_t wanted = (a.max_tokens + kTableThreads - 1) / kTableThreads;
+    const int64_t most = 2 * (int64_t)dev.sm_count;
+    const unsigned blocks = (unsigned)(wanted < 1 ? 1 : wanted > most ? most : wanted);
+    return launch(tables_kernel, blocks, kTableThreads, smem, stream, a);
+}
+
+template <typename Src, typename Dst, int kElems>
+static int launch_store(const spork_paged_store_args& a, DeviceState& dev, cudaStream_t stream)
+{
     const spork_paged_cache& c = a.cache;
-    if (slot < 0 || slot >= (int64_t)c.num_pages * c.page_size) {
-        return;
+    StoreShape shape;
+    shape.per_head = c.head_dim / kElems;
+    shape.items = 2 * c.kv_heads * shape.per_head;
+    shape.rows = shape.items < kStoreThreads ? kStoreThreads / shape.items : 1;
+    // Four tokens to a thread keep more loads under way, but leave SMs idle where there are few tokens: four once that
+    // fills the GPU's SMs with eight blocks each.
+    const int64_t blocks = (a.tokens + shape.rows - 1) / shape.rows;
+    if (blocks >= 4 * 8 * (int64_t)dev.sm_count) {
+        return launch(store_kernel<Src, Dst, kElems, 4>, (unsigned)((blocks + 3) / 4), kStoreThreads, 0, stream, a, shape);
     }
-    const int64_t page = slot / c.page_size, row = slot % c.page_size;
-    for (int i = threadIdx.x; i < c.kv_heads * c.head_dim; i += blockDim.x) {
-        const int h = i / c.head_dim, d = i % c.head_dim;
-        const Src k = static_cast<const Src*>(a.k)[t * a.k_token_stride + h * a.k_head_stride + d];
-        const Src v = static_cast<const Src*>(a.v)[t * a.v_token_stride + h * a.v_head_stride + d];
-        static_cast<Dst*>(c.k)[page * c.k_strides[0] + h * c.k_strides[1] + row * c.k_strides[2] + d] = round_to<Dst>(k);
-        static_cast<Dst*>(c.v)[page * c.v_strides[0] + h * c.v_strides[1] + row * c.v_strides[2] + d] = round_to<Dst>(v);
+    return launch(store_kernel<Src, Dst, kElems, 1>, (unsigned)blocks, kStoreThreads, 0, stream, a, shape);
+}
+
+// Whether all pieces of 8 elements lie on the boundaries that the wide loads and stores need.
+static bool store_aligned(const spork_paged_store_args& a)
+{
+    const spork_paged_cache& c = a.cache;
+    const int64_t src = a.src_type == SPORK_TYPE_F32 ? 4 : 8;  // elements of 16 bytes
+    int64_t any = c.head_dim & 7;
+    for (const void* p : {(const void*)c.k, (const void*)c.v, a.k, a.v}) {
+        any |= (int64_t)(reinterpret_cast<uintptr_t>(p) & 15u);
     }
+    const int64_t sizes[3] = {c.num_pages, c.kv_heads, c.page_size};
+    for (int i = 0; i < 3; ++i) {
+        any |= sizes[i] > 1 ? (c.k_strides[i] | c.v_strides[i]) & 7 : 0;
+    }
+    any |= a.tokens > 1 ? (a.k_token_stride | a.v_token_stride) & (src - 1) : 0;
+    any |= c.kv_heads > 1 ? (a.k_head_stride | a.v_head_stride) & (src - 1) : 0;
+    return any == 0;
 }
 
 template <typename Src, typename Dst>
-static int launch_store(const spork_paged_store_args& a, cudaStream_t stream)
+static int launch_store_types(const spork_paged_store_args& a, DeviceState& dev, cudaStream_t stream)
 {
-    store_kernel<Src, Dst><<<(unsigned)a.tokens, 256, 0, stream>>>(a);
-    return (int)cudaGetLastError();
+    return store_aligned(a) ? launch_store<Src, Dst, 8>(a, dev, stream) : launch_store<Src, Dst, 1>(a, dev, stream);
 }
 
 }  // namespace paged_sm100
@@ -173,8 +392,7 @@ extern "C" int spork_paged_sm100_tables(const spork_paged_tables_args* args, voi
         return rc;
     }
     using namespace spork::paged_sm100;
-    tables_kernel<<<1, kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return (int)cudaGetLastError();
+    return launch_tables(a, *dev, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int spork_paged_sm100_store(const spork_paged_store_args* args, void* stream)
@@ -212,8 +430,9 @@ extern "C" int spork_paged_sm100_store(const spork_paged_store_args* args, void*
     using namespace spork::paged_sm100;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a.cache.type == SPORK_TYPE_F16) {
-        return a.src_type == SPORK_TYPE_F32 ? launch_store<float, __half>(a, s) : launch_store<__half, __half>(a, s);
+        return a.src_type == SPORK_TYPE_F32 ? launch_store_types<float, __half>(a, *dev, s)
+                                            : launch_store_types<__half, __half>(a, *dev, s);
     }
-    return a.src_type == SPORK_TYPE_F32 ? launch_store<float, __nv_bfloat16>(a, s)
-                                        : launch_store<__nv_bfloat16, __nv_bfloat16>(a, s);
+    return a.src_type == SPORK_TYPE_F32 ? launch_store_types<float, __nv_bfloat16>(a, *dev, s)
+                                        : launch_store_types<__nv_bfloat16, __nv_bfloat16>(a, *dev, s);
 }

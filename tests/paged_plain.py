@@ -14,7 +14,7 @@ def tables(lengths, new, table, free, used, page, max_tokens):
         begin, tokens = tokens, tokens + adds
         offsets.append(min(begin, INT_MAX))
         width = len(table[r])
-        sound = held >= 0 and added >= 0 and (adds == 0 or tokens <= max_tokens) and held + adds <= width * page
+        sound = held >= 0 and added >= 0 and (adds == 0 or tokens <= max_tokens) and held + adds <= min(width * page, INT_MAX)
         if not sound:
             refused += 1
             after.append(held)

@@ -79,6 +79,7 @@ def test_tables_far_numbers_and_odd_lists(sp, cuda):
     _run_tables(sp, cuda, [3, 16], [1, 1], [[1, -7], [2, -7]], [5, 6], -1, 16, 2)
     _run_tables(sp, cuda, [3, 16], [1, 4], [[-1, -7], [2, -7]], [-5, 6], 0, 16, 5)
     _run_tables(sp, cuda, [0], [3], [[-7]], [I32], 0, I32, 3)
+    _run_tables(sp, cuda, [I32 - 1, I32 - 1, I32], [1, 2, 0], [[4, -7]] * 3, [I32, 8], 0, I32, 3)
     _run_tables(sp, cuda, [0, 0], [0, 0], [[], []], [], 0, 16, 2)
 
 
