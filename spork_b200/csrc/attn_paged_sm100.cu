@@ -2,25 +2,27 @@
 //   o[r][h] = softmax(scale q[r][h] K^T) V over the keys that request r holds, key head h / (heads / kv_heads).
 //
 // Every key and value is read once and used by the few query heads that share it, so the kernel is bound by HBM; the
-// products are small.  Work is cut along the cache: units of 64 keys of one (request, key head), all units in one list,
-// request by request, and each block of the grid takes an equal run of that list, whatever the lengths (they are known
-// on the device only).  A block joins what it computes of one (request, key head) and writes the result if it has all
-// of it; otherwise a partial result (running maximum, sum, unnormalised output) goes to the workspace, and a second
-// small kernel joins the parts in the order of the keys.  A block has at most two partial results: its first run and its
-// last one.
+// products are small.  Work is cut along the cache: units of 64 keys (128 with a head dimension of 64: 32 KB of keys and
+// values) of one (request, key head), all units in one list, request by request, and each block of the grid takes an
+// equal run of that list, whatever the lengths (they are known on the device only).  A block joins what it computes of
+// one (request, key head) and writes the result if it has all of it; otherwise a partial result (running maximum, sum,
+// unnormalised output) goes to the workspace, and a second small kernel joins the parts in the order of the keys.  A
+// block has at most two partial results: its first run and its last one.
 //
 // One warp copies the pages with TMA: the cache is a 5-dimensional tensor (64 elements, page rows, halves of the head
 // dimension, heads, pages) with the strides that it has, so any order in memory is one tensor map; a box is a page's
 // rows of one head (64 rows of it at most), swizzled for ldmatrix.  Page numbers come from the block table, and are
 // checked before they are used.
 //
-// The other warps compute, each on its own 16 (or 32) keys of a unit, with mma.m16n8k16.  Up to 8 query heads are rows
-// 0-7 of the 16-row operand, and rows 8-15 hold what rounding to 16 bits left over: of q, if it is fp32, and of the
-// softmax weights.  So both products are taken with about 22 (fp16) or 16 (bf16) bits of q and of the weights at no
-// cost: the rows would have been empty, and the weights' rounding, the largest error of the usual scheme, is gone.
-// Each warp runs its own online softmax, and the warps of a block are joined once per run, not once per unit.
-// (tcgen05 would want 64 or 128 rows and a trip through tensor memory for every unit; the warp instruction's rate is
-// several times what the loads can feed.)
+// Four warps compute, each on keys of its own, with mma.m16n8k16.  Up to 8 query heads are rows 0-7 of the 16-row
+// operand, and rows 8-15 hold what rounding to 16 bits left over: of q, if it is fp32, and of the softmax weights.  So
+// both products are taken with about 22 (fp16) or 16 (bf16) bits of q and of the weights at no cost: the rows would have
+// been empty, and the weights' rounding, the largest error of the usual scheme, is gone.  (tcgen05 would want 64 or 128
+// rows and a trip through tensor memory for every unit; the warp instruction's rate is several times what the loads can
+// feed.)  With 9 or more query heads to a key head the warps form 2 or 4 groups that share the unit, 8 heads each.
+// Each warp runs its own online softmax.  Its maximum follows the scores lazily: only when one has grown by more than
+// 2^8 over it are the row's lanes asked and the sums rescaled, so most units need no exchange between lanes at all.  The
+// warps of a group are joined once per (request, key head), pairwise: a warp that has handed its sums over goes on.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -42,29 +44,31 @@ namespace attn_paged_sm100 {
 using namespace spork::paged_sm100;
 using namespace spork::ptx;
 
-constexpr int kTile = 64;          // keys per unit
 constexpr int kHeads = 8;          // query heads of a group of warps
-constexpr int kPadded = 72;        // floats between the rows of the joining buffer (64 columns): no bank conflicts
-constexpr float kShift = 8.0f;     // weights are 2^(x - max + 8): up to 2^8, so that fp16 keeps the small ones normal
+// weights are 2^(x - max + 6), and max may be out of date by 8: up to 2^14, within fp16, whose small weights stay normal
+constexpr float kShift = 6.0f, kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMaxBlocks = 1024;   // blocks of a launch that a joined result can have parts from
-constexpr int kJoinThreads = 256;
+constexpr int kMaxBlocks = 1024;   // blocks of a launch
+constexpr int kComputeWarps = 4;
+constexpr int kThreads = (kComputeWarps + 1) * 32;
+constexpr int kBlocksPerSm = 2;
+constexpr int kPairCost = 1;       // what a (request, key head) costs a block besides its units, in units
+constexpr int kMaxRows = 64;       // rows of a TMA box
+constexpr int kJoinThreads = 128;
 
 // kGroups groups of warps share a unit, each with 8 query heads of its own.
 template <int D, int kGroups>
 struct Config {
-    static constexpr int kWarps = kGroups == 4 ? 2 : 4;         // warps of a group; each takes kTile / kWarps keys
+    static constexpr int kTile = 8192 / D;                      // keys per unit
+    static constexpr int kWarps = kComputeWarps / kGroups;      // warps of a group; each takes kTile / kWarps keys
     static constexpr int kKeys = kTile / kWarps;
-    static constexpr int kCompute = kGroups * kWarps;
-    static constexpr int kThreads = (kCompute + 1) * 32;
-    static constexpr int kBlocksPerSm = kGroups == 1 ? 2 : 1;
-    static constexpr int kHalves = D / 64;
+    static constexpr int kChunk = kKeys < 32 ? kKeys : 32;      // taken at once
     static constexpr int kHalfUnit = kTile * D * 2;             // the keys (or values) of a unit, bytes
     static constexpr int kStageBytes = 2 * kHalfUnit;
-    static constexpr int kStages = 96 * 1024 / kStageBytes * (kGroups == 1 ? 1 : 2);
-    static constexpr int kJoinFloats = kGroups * kWarps * kHeads * kPadded;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kJoinFloats * 4 + 1024;
-    static_assert(kSmem * kBlocksPerSm <= 227 * 1024 - 1024 * kBlocksPerSm, "shared memory");
+    static constexpr int kStages = 3;
+    static constexpr int kPadded = D + 8;                       // floats between the rows of the joining buffer: no bank conflicts
+    static constexpr int kJoinFloats = kGroups * (kWarps - 1) * kHeads * kPadded;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kJoinFloats * 4;
 };
 
 struct Params {
@@ -77,6 +81,7 @@ struct Params {
     int32_t requests, heads, kv_heads, group, head_units;  // group: query heads per key head; head_units: units along them
     int32_t max_blocks, num_pages, page_size, box_rows;
     float scale_log2e;
+    bool q_pairs;  // two neighbouring elements of q may be read at once
     // workspace
     int4* joins;       // per block: {request (-1: none), key head and head unit, last block, slot of the first part}
     float2* part_ml;   // [block][slot][head of the unit]: maximum, sum
@@ -85,49 +90,59 @@ struct Params {
 };
 
 struct Bars {
-    uint64_t full[16];
-    uint64_t empty[16];
-    int64_t warp_sums[16];
-    int32_t bad[16];       // per stage: a page outside the cache
-    int32_t start[3];      // request, head unit, unit of the block's first key
+    uint64_t full[4];
+    uint64_t empty[4];
+    int64_t warp_sums[8];
+    int64_t start_base;    // the list's position of the block's first (request, head unit)
+    int32_t start[2];      // which one that is
+    int32_t bad[4];        // per stage: a page outside the cache
+    float2 ml[kComputeWarps][kHeads];
     uint32_t abort_flag;
-    float2 ml[4 * 8 * kHeads / 2];
 };
-static_assert(sizeof(Bars) <= 1024 + 512, "barriers");
+static_assert(2 * (Config<128, 1>::kSmem + (int)sizeof(Bars) + 1024) <= 228 * 1024, "two blocks to an SM");
 
 // Units of a request: none if there is nothing to read, or nothing that may be read.
+template <int kTile>
 __device__ __forceinline__ int units_of(const Params& p, int r)
 {
     const int64_t len = p.lengths[r];
     return len > 0 && len <= (int64_t)p.max_blocks * p.page_size ? (int)((len + kTile - 1) / kTile) : 0;
 }
 
-// A block's run through the list of units, one (request, head unit) after the other.
+// A block's run through the list, one (request, head unit) after the other.  Each takes its units' places in the list
+// and kPairCost more.
+template <int kTile>
 struct Walk {
     int r, hh, first, count, units, len;
-    int64_t left;
+    int64_t base, end;  // places in the list: of the current one's first unit, of the end of the run
+    bool any;           // whether the block has had units before the current ones
 
-    __device__ __forceinline__ void here(const Params& p)
+    __device__ __forceinline__ void here(const Params& p, int64_t from)
     {
         len = p.lengths[r];
-        units = (len + kTile - 1) / kTile;
-        count = units - first < left ? units - first : (int)left;
+        units = (int)(((int64_t)len + kTile - 1) / kTile);
+        first = from > base ? (int)(from - base) : 0;
+        const int64_t last = end - base < units ? end - base : units;
+        count = last > first ? (int)(last - first) : 0;
     }
     // to the next one; false at the run's end
     __device__ __forceinline__ bool next(const Params& p)
     {
-        left -= count;
-        if (left <= 0) {
+        any = any || count > 0;
+        base += units + kPairCost;
+        if (base >= end) {
             return false;
         }
-        first = 0;
         if (++hh == p.kv_heads * p.head_units) {
             hh = 0;
             do {
                 ++r;
-            } while (units_of(p, r) == 0);
+                if (r >= p.requests) {
+                    return false;
+                }
+            } while (units_of<kTile>(p, r) == 0);
         }
-        here(p);
+        here(p, base);
         return true;
     }
 };
@@ -178,32 +193,163 @@ __device__ __forceinline__ void report_timeout(const Params& p, volatile uint32_
     atomicCAS(p.status, 0u, 0x90000000u | (role << 24) | ((where & 0xFFu) << 16) | (blockIdx.x & 0xFFFFu));
 }
 
+// Two neighbouring elements of q as 32-bit numbers; `pairs`: they may be read at once.
+template <typename Q>
+__device__ __forceinline__ float2 load_two(const Q* q, bool pairs)
+{
+    if (pairs) {
+        if constexpr (std::is_same<Q, float>::value) {
+            return *reinterpret_cast<const float2*>(q);
+        } else {
+            return unpack<Q>(*reinterpret_cast<const uint32_t*>(q));
+        }
+    }
+    return make_float2(to_f32(q[0]), to_f32(q[1]));
+}
+
+// Asks for the line of an address in L1 without waiting for it.
+__device__ __forceinline__ void touch(const void* p)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .u16 unused;\n\t"
+        "ld.global.ca.u16 unused, [%0];\n\t"
+        "}" ::"l"(p));
+}
+
+// What one warp has of its 8 query heads and a run of keys: maxima, sums, unnormalised output (fragments: row g of the
+// first product's operand is in [0], [1], row g + 8, its low part, in [2], [3]).
+template <int D, typename T, bool kLowQ, int kChunk>
+struct Softmax {
+    static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int kSteps = D / 16, kPairs = kChunk / 16;
+    uint32_t q_hi[kSteps][2], q_lo[kLowQ ? kSteps : 1][2];
+    float acc[D / 8][4];
+    float m, l;  // of row g; l: this lane's columns only
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+        }
+        m = -INFINITY;
+        l = 0.0f;
+    }
+
+    // kChunk keys, whose rows for ldmatrix are at k_row and v_row; `keys` of them count (kRagged: not all, and the rest
+    // may be anything).
+    template <bool kRagged>
+    __device__ __forceinline__ void add(const uint32_t (&k_row)[kPairs], const uint32_t (&v_row)[kPairs], uint32_t half,
+                                        int keys, float scale)
+    {
+        const int lane = threadIdx.x % 32, t = lane % 4, matrix = lane / 8, row8 = lane % 8;
+        float s[2 * kPairs][4];
+#pragma unroll
+        for (int i = 0; i < 2 * kPairs; ++i) {
+            s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+            for (int n = 0; n < kPairs; ++n) {
+                uint32_t b[4];
+                ldmatrix_x4(k_row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix % 2) ^ row8) << 4), b);
+                const uint32_t a1 = kLowQ ? q_lo[kLowQ ? i : 0][0] : 0u, a3 = kLowQ ? q_lo[kLowQ ? i : 0][1] : 0u;
+                mma_m16n8k16<kBf16>(s[2 * n], q_hi[i][0], a1, q_hi[i][1], a3, b[0], b[1]);
+                mma_m16n8k16<kBf16>(s[2 * n + 1], q_hi[i][0], a1, q_hi[i][1], a3, b[2], b[3]);
+            }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2 * kPairs; ++n) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x = s[n][j];
+                if (kLowQ) {
+                    // (a low part that is not finite has met an infinite key: the high part says what that gives)
+                    x += fabsf(s[n][2 + j]) < INFINITY ? s[n][2 + j] : 0.0f;
+                }
+                if (kRagged && n * 8 + 2 * t + j >= keys) {
+                    x = -INFINITY;
+                }
+                s[n][j] = x;
+                most = fmaxf(most, x);
+            }
+        }
+        most *= scale;
+        if (__any_sync(0xFFFFFFFFu, most > m + kSlack)) {
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+            most = fmaxf(most, m);
+            const float down = ex2(m - (most == -INFINITY ? 0.0f : most));
+            m = most;
+            l *= down;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                acc[i][0] *= down;
+                acc[i][1] *= down;
+                acc[i][2] *= down;
+                acc[i][3] *= down;
+            }
+        }
+        const float shift = m == -INFINITY ? 0.0f : kShift - m;
+#pragma unroll
+        for (int n = 0; n < kPairs; ++n) {
+            float w[4];
+            uint32_t a[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = ex2(fmaf(s[2 * n + j / 2][j % 2], scale, shift));
+                l += w[j];
+            }
+            split<T>(w[0], w[1], a[0], a[1]);
+            split<T>(w[2], w[3], a[2], a[3]);
+            // a value that does not count may be NaN, and its weight of zero would not remove it
+            uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
+            if (kRagged) {
+                const int k = n * 16 + 2 * t;
+                keep0 = (k < keys ? 0xFFFFu : 0u) | (k + 1 < keys ? 0xFFFF0000u : 0u);
+                keep1 = (k + 8 < keys ? 0xFFFFu : 0u) | (k + 9 < keys ? 0xFFFF0000u : 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                uint32_t b[4];
+                ldmatrix_x4_trans(v_row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix / 2) ^ row8) << 4), b);
+                mma_m16n8k16<kBf16>(acc[2 * i], a[0], a[1], a[2], a[3], kRagged ? b[0] & keep0 : b[0],
+                                    kRagged ? b[1] & keep1 : b[1]);
+                mma_m16n8k16<kBf16>(acc[2 * i + 1], a[0], a[1], a[2], a[3], kRagged ? b[2] & keep0 : b[2],
+                                    kRagged ? b[3] & keep1 : b[3]);
+            }
+        }
+    }
+};
+
 template <int D, typename T, typename Q, int kGroups>
-__global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroups>::kBlocksPerSm)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     attn_paged_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p)
 {
     using Cfg = Config<D, kGroups>;
-    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    using W = Walk<Cfg::kTile>;
     constexpr bool kLowQ = std::is_same<Q, float>::value;  // q has a low part
     constexpr int kUnitHeads = kGroups * kHeads;
     extern __shared__ uint8_t smem_raw[];
+    __shared__ Bars bars;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* behind = smem_raw + (stages - smem_u32(smem_raw)) + Cfg::kStages * Cfg::kStageBytes;
-    float* join = reinterpret_cast<float*>(behind);
-    __shared__ Bars bars;
+    float* join = reinterpret_cast<float*>(smem_raw + (stages - smem_u32(smem_raw)) + Cfg::kStages * Cfg::kStageBytes);
     volatile uint32_t* abort_flag = &bars.abort_flag;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(smem_u32(&bars.full[s]), 1);
-            mbar_init(smem_u32(&bars.empty[s]), Cfg::kCompute);
+            mbar_init(smem_u32(&bars.empty[s]), kComputeWarps);
             bars.bad[s] = 0;
         }
         bars.abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == Cfg::kCompute && lane == 0) {
+    if (warp == kComputeWarps && lane == 0) {
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
     }
@@ -211,17 +357,22 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
     grid_dependency_wait();
     grid_launch_dependents();
 
-    // ------------------------------------------------------------ this block's run of the list of units
+    // ------------------------------------------------------------ this block's run of the list
     const int hhs = p.kv_heads * p.head_units;
-    int64_t total = 0;
+    int64_t total = 0;  // places in the list
     {
-        const int chunk = (p.requests + Cfg::kThreads - 1) / Cfg::kThreads;
+        const int chunk = (p.requests + kThreads - 1) / kThreads;
         const int r0 = (int)threadIdx.x * chunk, r1 = r0 + chunk < p.requests ? r0 + chunk : p.requests;
+        const auto places = [&](int r) {
+            const int units = units_of<Cfg::kTile>(p, r);
+            return units ? (int64_t)(units + kPairCost) * hhs : 0;
+        };
         int64_t mine = 0;
         for (int r = r0; r < r1; ++r) {
-            mine += units_of(p, r);
+            mine += places(r);
         }
         int64_t upto = mine;
+#pragma unroll
         for (int d = 1; d < 32; d *= 2) {
             const int64_t w = __shfl_up_sync(0xFFFFFFFFu, upto, d);
             upto += lane >= d ? w : 0;
@@ -230,81 +381,104 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
             bars.warp_sums[warp] = upto;
         }
         __syncthreads();
-        int64_t before = 0;
-        for (int w = 0; w < Cfg::kThreads / 32; ++w) {
-            before += w < warp ? bars.warp_sums[w] : 0;
+        int64_t base = upto - mine;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            base += w < warp ? bars.warp_sums[w] : 0;
             total += bars.warp_sums[w];
         }
-        total *= hhs;
         const int64_t blocks = total < gridDim.x ? total : gridDim.x;
-        int64_t base = (before + upto - mine) * hhs;
         if (blockIdx.x < blocks) {
             const int64_t u0 = blockIdx.x * total / blocks;
-            if (u0 >= base && u0 < base + mine * hhs) {
-                int r = r0, units = units_of(p, r);
-                while (u0 >= base + (int64_t)units * hhs) {
-                    base += (int64_t)units * hhs;
-                    units = units_of(p, ++r);
+            if (u0 >= base && u0 < base + mine) {
+                int r = r0;
+                int64_t its = places(r);
+                while (u0 >= base + its) {
+                    base += its;
+                    its = places(++r);
                 }
+                const int hh = (int)((u0 - base) / (its / hhs));
                 bars.start[0] = r;
-                bars.start[1] = (int)((u0 - base) / units);
-                bars.start[2] = (int)((u0 - base) % units);
+                bars.start[1] = hh;
+                bars.start_base = base + hh * (its / hhs);
             }
         }
         __syncthreads();
     }
     const int64_t blocks = total < gridDim.x ? total : gridDim.x;
-    const int64_t u0 = blocks ? blockIdx.x * total / blocks : 0, u1 = blocks ? (blockIdx.x + 1) * total / blocks : 0;
-    Walk walk{};
-    walk.left = blockIdx.x < blocks ? u1 - u0 : 0;
-    if (walk.left > 0) {
+    const bool work = blockIdx.x < blocks;
+    W walk{};
+    if (work) {
         walk.r = bars.start[0];
         walk.hh = bars.start[1];
-        walk.first = bars.start[2];
-        walk.here(p);
+        walk.base = bars.start_base;
+        walk.end = (blockIdx.x + 1) * total / blocks;
+        walk.here(p, blockIdx.x * total / blocks);
     }
-    if (threadIdx.x == 0 && p.joins) {
-        // the block whose run is the second one with keys of a (request, head unit) names the parts of it
+    if (threadIdx.x == 0) {
+        // The first block whose run begins after the first unit of a (request, head unit), and before its end, names the
+        // parts of it: the block before has the first one (as its first run of units or a later one), then this block and
+        // those behind it as their first.
         int4 j = make_int4(-1, 0, 0, 0);
-        if (walk.left > 0 && walk.first > 0) {
-            const int64_t begin = u0 - walk.first, end = begin + walk.units, previous = (blockIdx.x - 1) * total / blocks;
-            if (previous <= begin) {
-                j = make_int4(walk.r, walk.hh, (int)((end * blocks - 1) / total), previous == begin ? 0 : 1);
+        if (work && walk.first > 0 && walk.count > 0) {
+            const int64_t previous = (blockIdx.x - 1) * total / blocks;
+            if (previous <= walk.base) {
+                const int64_t last = walk.base + walk.units - 1;
+                j = make_int4(walk.r, walk.hh, (int)(((last + 1) * blocks - 1) / total),
+                              previous >= walk.base - kPairCost ? 0 : 1);
             }
         }
         p.joins[blockIdx.x] = j;
     }
 
     const int rows = p.box_rows;
-    if (warp == Cfg::kCompute) {
+    if (warp == kComputeWarps) {
         // -------------------------------------------------------------------------------------- copies
         const Checker ck{p.status, stages, stages + Cfg::kStages * Cfg::kStageBytes, 0, 0};
-        const int boxes = kTile / rows;
+        const int boxes = Cfg::kTile / rows;
         const uint32_t box_bytes = rows * D * 2;
         uint32_t stage = 0, phase = 0, used = 0;
         bool ok = true;
-        bool more = walk.left > 0;
+        // to the first (request, head unit) from here on that has units for this block
+        auto settle = [&](bool more) {
+            while (more && walk.count == 0) {
+                more = walk.next(p);
+            }
+            return more;
+        };
+        bool more = settle(work);
         int unit = walk.first;
         // the page of this lane's box of a unit; -1 if it is behind the last key
-        auto page_of = [&](const Walk& w, int u) {
-            const int at = u * kTile + lane * rows;
-            return lane < boxes && at < w.len ? p.table[w.r * p.table_stride + at / p.page_size] : -1;
+        auto page_of = [&](int u) {
+            const int64_t at = (int64_t)u * Cfg::kTile + lane * rows;
+            return lane < boxes && at < walk.len ? p.table[walk.r * p.table_stride + (uint32_t)at / (uint32_t)p.page_size] : -1;
         };
-        int page = more ? page_of(walk, unit) : -1;
-        while (more && ok) {
-            const int at = unit * kTile + lane * rows;
+        int page = more ? page_of(unit) : -1;
+        while (more) {
+            const int64_t at = (int64_t)unit * Cfg::kTile + lane * rows;
             const bool mine = lane < boxes && at < walk.len;
             const int this_page = page, head = walk.hh / p.head_units;
+            const int row = mine ? (int)((uint32_t)at % (uint32_t)p.page_size) : 0;
             if (++unit == walk.first + walk.count) {
-                more = walk.next(p);
+                more = settle(walk.next(p));
                 unit = walk.first;
-            }
-            page = more ? page_of(walk, unit) : -1;  // asked for one unit ahead
-            if (!mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag)) {
-                if (lane == 0) {
-                    report_timeout(p, abort_flag, 1, stage);
+                if (more) {
+                    // the queries of what comes next, on their way while the units before it are worked on: a line per lane
+                    constexpr int kLines = D * (int)sizeof(Q) / 128;
+                    for (int i = lane; i < kUnitHeads * kLines; i += 32) {
+                        const int in_group = (walk.hh % p.head_units) * kUnitHeads + i / kLines;
+                        if (in_group < p.group) {
+                            touch(static_cast<const Q*>(p.q) + walk.r * p.q_request_stride +
+                                  (int64_t)(walk.hh / p.head_units * p.group + in_group) * p.q_head_stride +
+                                  (i % kLines) * (128 / (int)sizeof(Q)));
+                        }
+                    }
                 }
-                ok = false;
+            }
+            page = more ? page_of(unit) : -1;  // asked for one unit ahead
+            ok = mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag);
+            if (!ok && lane == 0) {
+                report_timeout(p, abort_flag, 1, stage);
             }
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) {
@@ -320,9 +494,9 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
             }
             __syncwarp();
             if (good && ck.smem(keys, box_bytes, 1024, 0x501) && ck.smem(keys + Cfg::kHalfUnit, box_bytes, 1024, 0x502) &&
-                ck.tma_coords(0, 2, at % p.page_size, this_page, 0x503)) {
-                tma_load_5d(keys, &map_k, full, 0, at % p.page_size, 0, head, this_page);
-                tma_load_5d(keys + Cfg::kHalfUnit, &map_v, full, 0, at % p.page_size, 0, head, this_page);
+                ck.tma_coords(0, 2, row, this_page, 0x503)) {
+                tma_load_5d(keys, &map_k, full, 0, row, 0, head, this_page);
+                tma_load_5d(keys + Cfg::kHalfUnit, &map_v, full, 0, row, 0, head, this_page);
             }
             ++used;
             if (++stage == Cfg::kStages) {
@@ -345,27 +519,31 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
         const int group = warp / Cfg::kWarps, part = warp % Cfg::kWarps;  // group of warps, warp of the group
         const int g = lane / 4, t = lane % 4;                             // row (query head) and column pair of a fragment
         const int matrix = lane / 8, row8 = lane % 8;
-        constexpr int kPairs = Cfg::kKeys / 16;                           // 16-key steps of a warp
-        constexpr int kSteps = D / 16;
+        using S = Softmax<D, T, kLowQ, Cfg::kChunk>;
+        constexpr int kPairs = S::kPairs, kSteps = S::kSteps, kChunks = Cfg::kKeys / Cfg::kChunk;
         // shared-memory offsets of this lane's ldmatrix rows: keys (matrices 0, 1 | 2, 3 are keys 0-7 | 8-15) and values
         // (matrices 0, 2 | 1, 3); a box of `rows` rows holds its halves of 64 columns one behind the other
         auto row_at = [&](int r) { return (uint32_t)((r / rows) * rows * D * 2 + (r % rows) * 128); };
-        uint32_t k_row[kPairs], v_row[kPairs];
-        for (int i = 0; i < kPairs; ++i) {
-            k_row[i] = row_at(part * Cfg::kKeys + i * 16 + (matrix / 2) * 8 + row8);
-            v_row[i] = row_at(part * Cfg::kKeys + i * 16 + (matrix % 2) * 8 + row8) + Cfg::kHalfUnit;
+        uint32_t k_at[kChunks][kPairs], v_at[kChunks][kPairs];
+        for (int c = 0; c < kChunks; ++c) {
+            for (int i = 0; i < kPairs; ++i) {
+                const int r = part * Cfg::kKeys + c * Cfg::kChunk + i * 16 + row8;
+                k_at[c][i] = row_at(r + (matrix / 2) * 8);
+                v_at[c][i] = row_at(r + (matrix % 2) * 8) + Cfg::kHalfUnit;
+            }
         }
         const uint32_t half = rows * 128;
-        float* my_join = join + (group * Cfg::kWarps + part) * kHeads * kPadded;
-        float2* group_ml = bars.ml + group * Cfg::kWarps * kHeads;
         uint32_t stage = 0, phase = 0;
-        bool ok = true;
+        bool ok = true, joined = false;
+        S sm;
 
-        for (bool more = walk.left > 0; more; more = walk.next(p)) {
+        for (bool more = work; more; more = walk.next(p)) {
+            if (walk.count == 0) {
+                continue;
+            }
             const int kv = walk.hh / p.head_units, in_group = (walk.hh % p.head_units) * kUnitHeads + group * kHeads + g;
             const bool head_here = in_group < p.group;
             // q: rows g and, for what rounding left over, g + 8 of the A operand
-            uint32_t q_hi[kSteps][2], q_lo[kLowQ ? kSteps : 1][2];
             {
                 const Q* q = static_cast<const Q*>(p.q) + walk.r * p.q_request_stride +
                              (int64_t)(kv * p.group + (head_here ? in_group : 0)) * p.q_head_stride + 2 * t;
@@ -373,23 +551,18 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
                 for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float x = head_here ? to_f32(q[i * 16 + j * 8]) : 0.0f;
-                        const float y = head_here ? to_f32(q[i * 16 + j * 8 + 1]) : 0.0f;
+                        float2 x = load_two(q + i * 16 + j * 8, p.q_pairs);
+                        x = head_here ? x : make_float2(0.0f, 0.0f);
                         if (kLowQ) {
-                            split<T>(x, y, q_hi[i][j], q_lo[kLowQ ? i : 0][j]);
+                            split<T>(x.x, x.y, sm.q_hi[i][j], sm.q_lo[kLowQ ? i : 0][j]);
                         } else {
-                            q_hi[i][j] = pack<T>(x, y);
+                            sm.q_hi[i][j] = pack<T>(x.x, x.y);
                         }
                     }
                 }
             }
-            float acc[D / 8][4];
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-            }
-            float m = -INFINITY, l = 0.0f;  // of row g; l: this lane's columns only
-            bool bad = false;
+            sm.clear();
+            int bad = 0;
 
             for (int u = walk.first; u < walk.first + walk.count; ++u) {
                 if (ok && !mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
@@ -397,88 +570,22 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
                     ok = false;
                 }
                 ok = __all_sync(0xFFFFFFFFu, ok);
-                bad = bad || *const_cast<volatile int32_t*>(&bars.bad[stage]) != 0;
-                const int first_key = u * kTile + part * Cfg::kKeys;
-                if (ok && first_key < walk.len) {
-                    const uint32_t base = stages + stage * Cfg::kStageBytes;
-                    // scores of Cfg::kKeys keys: 8 at a time
-                    float s[2 * kPairs][4];
+                bad |= *const_cast<volatile int32_t*>(&bars.bad[stage]);
+                const uint32_t base = stages + stage * Cfg::kStageBytes;
+                const int64_t left = walk.len - (int64_t)u * Cfg::kTile - part * Cfg::kKeys;  // keys from this warp's first on
 #pragma unroll
-                    for (int i = 0; i < 2 * kPairs; ++i) {
-                        s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+                for (int c = 0; c < kChunks; ++c) {
+                    uint32_t k_row[kPairs], v_row[kPairs];
+#pragma unroll
+                    for (int i = 0; i < kPairs; ++i) {
+                        k_row[i] = base + k_at[c][i];
+                        v_row[i] = base + v_at[c][i];
                     }
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-                        for (int n = 0; n < kPairs; ++n) {
-                            uint32_t b[4];
-                            ldmatrix_x4(base + k_row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix % 2) ^ row8) << 4), b);
-                            const uint32_t a1 = kLowQ ? q_lo[kLowQ ? i : 0][0] : 0u, a3 = kLowQ ? q_lo[kLowQ ? i : 0][1] : 0u;
-                            mma_m16n8k16<kBf16>(s[2 * n], q_hi[i][0], a1, q_hi[i][1], a3, b[0], b[1]);
-                            mma_m16n8k16<kBf16>(s[2 * n + 1], q_hi[i][0], a1, q_hi[i][1], a3, b[2], b[3]);
-                        }
-                    }
-                    const int keys = walk.len - first_key;  // that count; the rest may be anything
-                    const bool ragged = keys < Cfg::kKeys;
-                    float most = -INFINITY;
-#pragma unroll
-                    for (int n = 0; n < 2 * kPairs; ++n) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            float x = s[n][j];
-                            if (kLowQ) {
-                                // (a part that is not finite has met an infinite key: the high part says what it gives)
-                                x += fabsf(s[n][2 + j]) < INFINITY ? s[n][2 + j] : 0.0f;
-                            }
-                            x *= p.scale_log2e;
-                            if (ragged && n * 8 + 2 * t + j >= keys) {
-                                x = -INFINITY;
-                            }
-                            s[n][j] = x;
-                            most = fmaxf(most, x);
-                        }
-                    }
-                    most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-                    const float m_new = fmaxf(m, most);
-                    const float shift = m_new == -INFINITY ? 0.0f : m_new - kShift;
-                    if (__any_sync(0xFFFFFFFFu, m_new > m)) {
-                        const float down = ex2(m - (m_new == -INFINITY ? 0.0f : m_new));
-                        l *= down;
-#pragma unroll
-                        for (int i = 0; i < D / 8; ++i) {
-                            acc[i][0] *= down;
-                            acc[i][1] *= down;
-                            acc[i][2] *= down;
-                            acc[i][3] *= down;
-                        }
-                        m = m_new;
-                    }
-#pragma unroll
-                    for (int n = 0; n < kPairs; ++n) {
-                        float w[4];
-                        uint32_t a[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            w[j] = ex2(s[2 * n + j / 2][j % 2] - shift);
-                            l += w[j];
-                        }
-                        split<T>(w[0], w[1], a[0], a[1]);
-                        split<T>(w[2], w[3], a[2], a[3]);
-                        // a value that does not count may be NaN, and its weight of zero would not remove it
-                        uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
-                        if (ragged) {
-                            const int k = n * 16 + 2 * t;
-                            keep0 = (k < keys ? 0xFFFFu : 0u) | (k + 1 < keys ? 0xFFFF0000u : 0u);
-                            keep1 = (k + 8 < keys ? 0xFFFFu : 0u) | (k + 9 < keys ? 0xFFFF0000u : 0u);
-                        }
-#pragma unroll
-                        for (int i = 0; i < kSteps; ++i) {
-                            uint32_t b[4];
-                            ldmatrix_x4_trans(base + v_row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix / 2) ^ row8) << 4), b);
-                            mma_m16n8k16<kBf16>(acc[2 * i], a[0], a[1], a[2], a[3], b[0] & keep0, b[1] & keep1);
-                            mma_m16n8k16<kBf16>(acc[2 * i + 1], a[0], a[1], a[2], a[3], b[2] & keep0, b[3] & keep1);
-                        }
+                    const int keys = left > Cfg::kTile ? Cfg::kTile : (int)left - c * Cfg::kChunk;
+                    if (ok && keys >= Cfg::kChunk) {
+                        sm.template add<false>(k_row, v_row, half, keys, p.scale_log2e);
+                    } else if (ok && keys > 0) {
+                        sm.template add<true>(k_row, v_row, half, keys, p.scale_log2e);
                     }
                 }
                 __syncwarp();
@@ -492,87 +599,93 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
             }
 
             // ------------------------------------------------- the warps of the group joined, the result or part written
+            float o[D / 8][2], m = sm.m, l = sm.l;
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-            if (bad) {
-                l = NAN;
-            }
-            if (t == 0) {
-                group_ml[part * kHeads + g] = make_float2(m, l);
-            }
-            named_barrier_sync(1 + group, Cfg::kWarps * 32);
-            float m_all = -INFINITY;
+            l = bad ? NAN : l;
 #pragma unroll
-            for (int w = 0; w < Cfg::kWarps; ++w) {
-                m_all = fmaxf(m_all, group_ml[w * kHeads + g].x);
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] = sm.acc[i][0] + sm.acc[i][2];
+                o[i][1] = sm.acc[i][1] + sm.acc[i][3];
             }
-            const float down = ex2(m - (m_all == -INFINITY ? 0.0f : m_all));
-            const bool whole = walk.count == walk.units;
-            const int slot = walk.first > 0 || walk.left == u1 - u0 ? 0 : 1;
+            // Warps kWarps / 2 .. kWarps - 1 hand their sums to warps 0 .., and so on.  Named barriers of the two warps:
+            // 2 w - 1 says that warp w's buffer is full, 2 w that it is free again (w: among all compute warps).
+            bool mine = true;
 #pragma unroll
-            for (int c = 0; c < Cfg::kHalves; ++c) {
+            for (int from = Cfg::kWarps / 2; from > 0; from /= 2) {
+                if (part >= from && part < 2 * from) {
+                    float* to = join + ((group * (Cfg::kWarps - 1) + part - 1) * kHeads + g) * Cfg::kPadded + 2 * t;
+                    if (joined) {
+                        named_barrier_sync(2 * warp, 64);
+                    }
+                    if (t == 0) {
+                        bars.ml[warp][g] = make_float2(m, l);
+                    }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float* a = acc[c * 8 + i];
-                    *reinterpret_cast<float2*>(my_join + g * kPadded + i * 8 + 2 * t) =
-                        make_float2((a[0] + a[2]) * down, (a[1] + a[3]) * down);
+                    for (int i = 0; i < D / 8; ++i) {
+                        *reinterpret_cast<float2*>(to + i * 8) = make_float2(o[i][0], o[i][1]);
+                    }
+                    named_barrier_arrive(2 * warp - 1, 64);
+                    mine = false;
+                } else if (part < from) {
+                    const int other = warp + from;
+                    const float* at = join + ((group * (Cfg::kWarps - 1) + part + from - 1) * kHeads + g) * Cfg::kPadded + 2 * t;
+                    named_barrier_sync(2 * other - 1, 64);
+                    const float2 ml = bars.ml[other][g];
+                    const float most = fmaxf(m, ml.x), to = most == -INFINITY ? 0.0f : most;
+                    const float down = ex2(m - to), other_down = ex2(ml.x - to);
+                    l = l * down + ml.y * other_down;
+                    m = most;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        const float2 x = *reinterpret_cast<const float2*>(at + i * 8);
+                        o[i][0] = o[i][0] * down + x.x * other_down;
+                        o[i][1] = o[i][1] * down + x.y * other_down;
+                    }
+                    named_barrier_arrive(2 * other, 64);
                 }
-                named_barrier_sync(1 + group, Cfg::kWarps * 32);
-                // a thread takes four columns at a time
-                for (int i = part * 32 + lane; i < kHeads * 16; i += Cfg::kWarps * 32) {
-                    const int h = i / 16, column = (i % 16) * 4;
-                    const int head = (walk.hh % p.head_units) * kUnitHeads + group * kHeads + h;
-                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float m_h = -INFINITY, l_h = 0.0f;
+            }
+            joined = true;
+            if (mine && head_here) {
+                if (walk.count == walk.units) {
+                    const int64_t row = (int64_t)walk.r * p.heads + kv * p.group + in_group;
+                    const float by = 1.0f / l;
+                    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + row * D) + t;
 #pragma unroll
-                    for (int w = 0; w < Cfg::kWarps; ++w) {
-                        const float4 x = *reinterpret_cast<const float4*>(
-                            join + ((group * Cfg::kWarps + w) * kHeads + h) * kPadded + column);
-                        sum.x += x.x;
-                        sum.y += x.y;
-                        sum.z += x.z;
-                        sum.w += x.w;
-                        m_h = fmaxf(m_h, group_ml[w * kHeads + h].x);
+                    for (int i = 0; i < D / 8; ++i) {
+                        out[i * 4] = pack<T>(o[i][0] * by, o[i][1] * by);
                     }
-                    const float base = m_h == -INFINITY ? 0.0f : m_h;
+                    if (p.lse && t == 0) {
+                        p.lse[row] = ((m == -INFINITY ? 0.0f : m) - kShift + log2f(l)) * kLn2;
+                    }
+                } else {
+                    const int64_t row = ((int64_t)blockIdx.x * 2 + (walk.any ? 1 : 0)) * kUnitHeads + group * kHeads + g;
+                    float* out = p.part_o + row * D + 2 * t;
 #pragma unroll
-                    for (int w = 0; w < Cfg::kWarps; ++w) {
-                        const float2 ml = group_ml[w * kHeads + h];
-                        l_h += ml.y * ex2(ml.x - base);
+                    for (int i = 0; i < D / 8; ++i) {
+                        *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[i][0], o[i][1]);
                     }
-                    if (head < p.group) {
-                        if (whole) {
-                            const int64_t row = (int64_t)walk.r * p.heads + kv * p.group + head;
-                            const float by = 1.0f / l_h;
-                            uint2 out;
-                            out.x = pack<T>(sum.x * by, sum.y * by);
-                            out.y = pack<T>(sum.z * by, sum.w * by);
-                            *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + row * D + c * 64 + column) = out;
-                            if (p.lse && c == 0 && column == 0) {
-                                p.lse[row] = (base - kShift + log2f(l_h)) * kLn2;
-                            }
-                        } else {
-                            const int64_t row = ((int64_t)blockIdx.x * 2 + slot) * kUnitHeads + group * kHeads + h;
-                            *reinterpret_cast<float4*>(p.part_o + row * D + c * 64 + column) = sum;
-                            if (c == 0 && column == 0) {
-                                p.part_ml[row] = make_float2(m_h, l_h);
-                            }
-                        }
+                    if (t == 0) {
+                        p.part_ml[row] = make_float2(m, l);
                     }
                 }
-                named_barrier_sync(1 + group, Cfg::kWarps * 32);
             }
+            __syncwarp();
+        }
+        // the last buffers that were handed over have been taken (their barriers are left as they were found)
+        if (joined && part > 0) {
+            named_barrier_sync(2 * warp, 64);
         }
         // requests without units: no keys, or lengths that cannot be
         for (int r = blockIdx.x; r < p.requests; r += gridDim.x) {
-            if (units_of(p, r) == 0) {
+            if (units_of<Cfg::kTile>(p, r) == 0) {
                 const bool empty = p.lengths[r] == 0;
                 const uint32_t fill = empty ? 0u : pack<T>(NAN, NAN);
                 uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + (int64_t)r * p.heads * D);
-                for (int i = threadIdx.x; i < p.heads * (D / 2); i += Cfg::kCompute * 32) {
+                for (int i = threadIdx.x; i < p.heads * (D / 2); i += kComputeWarps * 32) {
                     o[i] = fill;
                 }
-                for (int i = threadIdx.x; p.lse && i < p.heads; i += Cfg::kCompute * 32) {
+                for (int i = threadIdx.x; p.lse && i < p.heads; i += kComputeWarps * 32) {
                     p.lse[(int64_t)r * p.heads + i] = empty ? -INFINITY : NAN;
                 }
             }
@@ -580,14 +693,15 @@ __global__ void __launch_bounds__(Config<D, kGroups>::kThreads, Config<D, kGroup
     }
 }
 
-// Joins the parts of one query head of a (request, head unit): block x of the first kernel named them in joins[x].
+// Joins the parts of one query head of a (request, head unit): block x of the first kernel named them in joins[x].  Most
+// blocks find nothing to join or a few parts, so a part is one warp's read and its maximum, sum and output are asked for
+// at once; of many parts each warp takes every fourth, and the warps are joined at the end.
 template <int D, typename T>
 __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Params p, int unit_heads)
 {
-    constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes;  // threads along a part's columns; parts at a time
-    __shared__ float weight[kMaxBlocks + 1];
-    __shared__ float2 seen[kJoinThreads / 32];
-    __shared__ float4 sums[kRows][kLanes];
+    constexpr int kWarps = kJoinThreads / 32, kPer = D / 32;
+    __shared__ float2 ml[kWarps];
+    __shared__ float sums[kWarps][D];
     grid_dependency_wait();
     grid_launch_dependents();
     const int4 j = p.joins[blockIdx.x];
@@ -596,72 +710,74 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Par
         return;
     }
     const int parts = j.z - (int)blockIdx.x + 2;  // of blocks blockIdx.x - 1 .. j.z
-    auto row_of = [&](int i) {
-        return (((int64_t)blockIdx.x - 1 + i) * 2 + (i == 0 ? j.w : 0)) * unit_heads + h;
-    };
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    float most = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
-        most = fmaxf(most, p.part_ml[row_of(i)].x);
-    }
-    for (int d = 16; d > 0; d /= 2) {
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+    float m = -INFINITY, l = 0.0f, o[kPer] = {};
+    constexpr int kAtOnce = 4;
+    for (int i0 = warp; i0 < parts; i0 += kAtOnce * kWarps) {
+        float2 part[kAtOnce];
+        float x[kAtOnce][kPer];
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+            const int i = i0 + n * kWarps;
+            if (i < parts) {
+                const int64_t row = (((int64_t)blockIdx.x - 1 + i) * 2 + (i == 0 ? j.w : 0)) * unit_heads + h;
+                part[n] = p.part_ml[row];
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    x[n][k] = p.part_o[row * D + lane + k * 32];
+                }
+            } else {
+                part[n] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    x[n][k] = 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+            const float most = fmaxf(m, part[n].x), to = most == -INFINITY ? 0.0f : most;
+            const float down = ex2(m - to), other = ex2(part[n].x - to);
+            m = most;
+            l = l * down + part[n].y * other;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                o[k] = o[k] * down + x[n][k] * other;
+            }
+        }
     }
     if (lane == 0) {
-        seen[warp].x = most;
+        ml[warp] = make_float2(m, l);
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        sums[warp][lane + k * 32] = o[k];
     }
     __syncthreads();
-    for (int w = 0; w < kJoinThreads / 32; ++w) {
-        most = fmaxf(most, seen[w].x);
+    float most = -INFINITY, total = 0.0f;
+    for (int w = 0; w < kWarps; ++w) {
+        most = fmaxf(most, ml[w].x);
     }
-    const float base = most == -INFINITY ? 0.0f : most;
-    float sum = 0.0f;
-    for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
-        const float2 ml = p.part_ml[row_of(i)];
-        weight[i] = ex2(ml.x - base);
-        sum += ml.y * weight[i];
+    const float to = most == -INFINITY ? 0.0f : most;
+    float weight[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        weight[w] = ex2(ml[w].x - to);
+        total += ml[w].y * weight[w];
     }
-    for (int d = 16; d > 0; d /= 2) {
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    }
-    if (lane == 0) {
-        seen[warp].y = sum;
-    }
-    __syncthreads();
-    sum = 0.0f;
-    for (int w = 0; w < kJoinThreads / 32; ++w) {
-        sum += seen[w].y;
-    }
-    const int column = threadIdx.x % kLanes, first = threadIdx.x / kLanes;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = first; i < parts; i += kRows) {
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + row_of(i) * D + column * 4);
-        const float w = weight[i];
-        v.x += x.x * w;
-        v.y += x.y * w;
-        v.z += x.z * w;
-        v.w += x.w * w;
-    }
-    sums[first][column] = v;
-    __syncthreads();
-    if (threadIdx.x < kLanes) {
-        for (int i = 1; i < kRows; ++i) {
-            const float4 x = sums[i][column];
-            v.x += x.x;
-            v.y += x.y;
-            v.z += x.z;
-            v.w += x.w;
+    const int64_t row = (int64_t)j.x * p.heads + (j.y / p.head_units) * p.group + head;
+    const float by = 1.0f / total;
+    if (threadIdx.x < D / 2) {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            a += sums[w][2 * threadIdx.x] * weight[w];
+            b += sums[w][2 * threadIdx.x + 1] * weight[w];
         }
-        const int64_t row = (int64_t)j.x * p.heads + (j.y / p.head_units) * p.group + head;
-        const float by = 1.0f / sum;
-        uint2 out;
-        out.x = pack<T>(v.x * by, v.y * by);
-        out.y = pack<T>(v.z * by, v.w * by);
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + row * D + column * 4) = out;
-        if (p.lse && threadIdx.x == 0) {
-            p.lse[row] = (base - kShift + log2f(sum)) * kLn2;
-        }
+        reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + row * D)[threadIdx.x] = pack<T>(a * by, b * by);
+    }
+    if (p.lse && threadIdx.x == 0) {
+        p.lse[row] = (to - kShift + log2f(total)) * kLn2;
     }
 }
 
@@ -688,7 +804,7 @@ static EncodeTiledFn encode_tiled_fn()
 
 // Query heads of a key head are taken 8, 16 or 32 at a time (groups of warps that share the keys in shared memory).
 static int groups_of(int group) { return group <= kHeads ? 1 : group <= 2 * kHeads ? 2 : 4; }
-static int blocks_of(int groups, int sm_count) { return (groups == 1 ? 2 : 1) * sm_count; }
+static int blocks_of(int sm_count) { return kBlocksPerSm * sm_count; }
 
 static int make_map(CUtensorMap* map, void* base, const spork_paged_cache& c, const int64_t* strides)
 {
@@ -702,7 +818,7 @@ static int make_map(CUtensorMap* map, void* base, const spork_paged_cache& c, co
                                 (cuuint64_t)(c.num_pages > 0 ? c.num_pages : 1)};
     const cuuint64_t steps[4] = {bytes(strides[2], c.page_size), 128, bytes(strides[1], c.kv_heads),
                                  bytes(strides[0], c.num_pages)};
-    const cuuint32_t box[5] = {64, (cuuint32_t)(c.page_size < kTile ? c.page_size : kTile), (cuuint32_t)(c.head_dim / 64), 1, 1};
+    const cuuint32_t box[5] = {64, (cuuint32_t)(c.page_size < kMaxRows ? c.page_size : kMaxRows), (cuuint32_t)(c.head_dim / 64), 1, 1};
     const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, c.type == SPORK_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                           base, dims, steps, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -750,9 +866,9 @@ static int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Para
     if (attr_err[dev.ordinal] != cudaSuccess) {
         return (int)attr_err[dev.ordinal];
     }
-    const int blocks = blocks_of(kGroups, dev.sm_count);
+    const int blocks = blocks_of(dev.sm_count);
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = launch_config(&attr, dim3(blocks), Cfg::kThreads, Cfg::kSmem, stream);
+    cudaLaunchConfig_t cfg = launch_config(&attr, dim3(blocks), kThreads, Cfg::kSmem, stream);
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p);
     if (e == cudaSuccess && joined) {
         const int heads = p.group < kGroups * kHeads ? p.group : kGroups * kHeads;
@@ -802,7 +918,7 @@ extern "C" int64_t spork_attn_sm100_paged_workspace(int heads, int kv_heads, int
         return -(int64_t)rc;
     }
     const int groups = groups_of(heads / kv_heads);
-    return Workspace(blocks_of(groups, dev->sm_count), groups, head_dim).bytes;
+    return Workspace(blocks_of(dev->sm_count), groups, head_dim).bytes;
 }
 
 extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* stream)
@@ -847,7 +963,7 @@ extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* s
     if (rc2) {
         return rc2;
     }
-    const int group = a.heads / c.kv_heads, groups = groups_of(group), blocks = blocks_of(groups, dev->sm_count);
+    const int group = a.heads / c.kv_heads, groups = groups_of(group), blocks = blocks_of(dev->sm_count);
     const Workspace w(blocks, groups, c.head_dim);
     if (blocks > kMaxBlocks) {
         return SPORK_ERR_TOO_LARGE;
@@ -878,15 +994,16 @@ extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* s
     p.max_blocks = a.max_blocks;
     p.num_pages = c.num_pages;
     p.page_size = c.page_size;
-    p.box_rows = c.page_size < kTile ? c.page_size : kTile;
+    p.box_rows = c.page_size < kMaxRows ? c.page_size : kMaxRows;
     p.scale_log2e = a.scale * kLog2e;
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     p.joins = reinterpret_cast<int4*>(ws + w.joins);
     p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
     p.part_o = reinterpret_cast<float*>(ws + w.o);
     p.status = dev->status_word;
+    p.q_pairs = ((reinterpret_cast<uintptr_t>(a.q) % (2 * q_elem)) | ((a.q_request_stride | a.q_head_stride) & 1)) == 0;
     // one unit at most for every request: nothing to join
-    const bool joined = (int64_t)a.max_blocks * c.page_size > kTile;
+    const bool joined = (int64_t)a.max_blocks * c.page_size > 8192 / c.head_dim;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f32 = a.q_type == SPORK_TYPE_F32;
     if (c.type == SPORK_TYPE_F16) {

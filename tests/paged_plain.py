@@ -64,15 +64,16 @@ def tolerances(dtype, keys, dim, ref, weighted, size, fp32_q):
     core may truncate) of the sum of their magnitudes; a 32-bit q is taken as two 16-bit parts, which leaves (eps / 2)^2 of
     it (for fp16 at least 2^-25 absolutely, a subnormal's half step, on q of a size around one: within the same bound
     times four); scaling, subtracting the maximum and the exponential add a few 2^-23 of the score's magnitude.  A score off by e moves a weight
-    by e and, through the sum, the others by e: 2 e of the weighted magnitudes.  Weights: taken as two 16-bit parts of
-    numbers up to 2^8, (eps / 2)^2, and a key whose weight is below the smallest step (2^-33 of the largest) by that much.
+    by e and, through the sum, the others by e: 2 e of the weighted magnitudes.  Weights: taken as two 16-bit parts,
+    (eps / 2)^2, of numbers that are 2^6 at least for the largest weight: a key whose weight is below half the smallest step
+    of fp16, 2^-25, is off by that much, 2^-31 of the largest.
     Sums over the keys: at most one step of 2^-23 for every key and joining, of the weighted magnitudes.  At the end o is
     rounded once: eps / 2 of its own value (below the normal range: half the smallest step)."""
     import torch
 
     half = torch.finfo(dtype).eps / 2
     e = size * ((dim + 8) * 2.0 ** -23 + (4 * half * half if fp32_q else 0.0)) + 2.0 ** -21
-    inner = 2 * e + half * half + keys * 2.0 ** -33 + (keys + 64) * 2.0 ** -23
+    inner = 2 * e + half * half + keys * 2.0 ** -31 + (keys + 64) * 2.0 ** -23
     tol_o = half * ref.abs() + (1 + half) * inner[:, None] * weighted + torch.finfo(dtype).smallest_normal * half
     tol_lse = e + (keys + 64) * 2.0 ** -23 + 2.0 ** -23 * (size + math.log(max(keys, 1)) + 1)
     return tol_o, tol_lse
