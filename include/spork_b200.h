@@ -434,10 +434,16 @@ int spork_paged_sm100_store(const spork_paged_store_args* args, void* stream);
  * page behind the last key, may hold anything.  head_dim 64 or 128; page_size 8, 16,
  * 32 or a multiple of 64; heads a multiple of kv_heads; k, v and their strides
  * multiples of 16 bytes; scale positive and finite.
+ * A value of V that is not finite makes what it counts in so too (NaN, where the
+ * definition may give an infinity); fp32 q has to lie within the cache type's range.
  * `workspace`: device memory of spork_attn_sm100_paged_workspace bytes, 16-byte
- * aligned, not read by anything else until the call has run; its contents before
- * and after do not matter.  Results do not depend on the timing of the run: they are
- * the same, bit for bit, in every run on the same kind of GPU. */
+ * aligned.  Its first SPORK_ATTN_PAGED_COUNTERS bytes must be zero before the first
+ * call that uses it, and every call leaves them so (unless it was given up half way:
+ * spork_gemm_sm100_status then reports it, and they are to be zeroed again); the rest
+ * may hold anything.  Calls that may run at the same time need a workspace each.
+ * Results do not depend on the timing of the run: they are the same, bit for bit, in
+ * every run on the same kind of GPU. */
+#define SPORK_ATTN_PAGED_COUNTERS 65536
 typedef struct spork_attn_paged_args {
     spork_paged_cache cache;
     const void* q;

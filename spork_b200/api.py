@@ -364,6 +364,7 @@ def status(stream=None, device=None) -> None:
         detail = ctypes.c_uint32(0)
         rc = lib().spork_gemm_sm100_status(_stream_ptr(stream), ctypes.byref(detail))
     if rc != 0:
+        _workspaces.clear()  # a launch that was given up may have left its counters as they were
         raise SporkError(rc, f"device status (detail 0x{detail.value:08x})")
 
 
@@ -471,7 +472,9 @@ _PAGED_ATTN_ARGS = struct.Struct("=" + _CACHE + "6Q4q4ifi")
 _T = None
 _TYPE_CODES: dict = {}
 _current_device = _raw_stream = None
-_workspace_bytes: dict = {}
+_workspace_bytes: dict = {}  # by device and what the size depends on
+_workspaces: dict = {}       # by device and stream: the one that calls without a workspace of their own use
+_COUNTER_BYTES = 65536       # SPORK_ATTN_PAGED_COUNTERS
 
 
 def _bind_torch():
@@ -519,6 +522,34 @@ def _new(like, shape, dtype, stream):
         return _T.empty(shape, dtype=dtype, device=like.device)
     with _T.cuda.stream(stream):
         return _T.empty(shape, dtype=dtype, device=like.device)
+
+
+def _workspace(like, device: int, need: int, stream):
+    """A workspace for one launch.  Launches of one stream follow one another and share the stream's; a captured launch, whose
+    graph may be replayed beside any other, gets one of its own, with the clearing of its counters in the graph."""
+    key = (device, _raw_stream(device) if stream is None else stream.cuda_stream)
+    if _T.cuda.is_current_stream_capturing() if stream is None else _capturing(stream):
+        workspace = _new(like, (need,), _T.uint8, stream)
+        if stream is None:
+            workspace[:_COUNTER_BYTES].zero_()
+        else:
+            with _T.cuda.stream(stream):
+                workspace[:_COUNTER_BYTES].zero_()
+        return workspace
+    workspace = _workspaces.get(key)
+    if workspace is None or workspace.numel() < need:
+        if stream is None:
+            workspace = _T.zeros((need,), dtype=_T.uint8, device=like.device)
+        else:
+            with _T.cuda.stream(stream):
+                workspace = _T.zeros((need,), dtype=_T.uint8, device=like.device)
+        _workspaces[key] = workspace
+    return workspace
+
+
+def _capturing(stream) -> bool:
+    with _T.cuda.stream(stream):
+        return _T.cuda.is_current_stream_capturing()
 
 
 def _vector(t, n, dtype, what: str):
@@ -663,8 +694,9 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     ``block_table`` (R, max_blocks) and ``lengths`` (R,) are int32.  ``o`` (contiguous) has the cache's type.  ``lse``, if
     given, is (R, heads) float32 and receives the logarithm of each softmax's sum.  A request of length 0 gets zeros (lse
     -inf); one with a length outside its table row or a page outside the cache gets NaN.  ``workspace`` is a contiguous
-    CUDA tensor of attn_paged_workspace bytes, allocated for the call if it is not given; launches that may run at the same
-    time (other streams, other captured graphs) need one each."""
+    CUDA tensor of attn_paged_workspace bytes, zero when it is first used and left so by every call; launches that may run at
+    the same time (other streams, other captured graphs) need one each.  Without one, a stream's launches share one that is
+    kept for the stream, and a captured launch gets its own."""
     torch = _T or _bind_torch()
     q_shape = q.shape
     if len(q_shape) != 3:
@@ -707,7 +739,8 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
         if need is None:
             with _OnDevice(device):
                 need = _workspace_bytes[key] = attn_paged_workspace(heads, kv_heads, dim)
-        workspace = _new(q, (need,), torch.uint8, stream)
+        workspace = _workspace(q, device, need, stream)
+        need = workspace.numel()
     else:
         need = workspace.numel() * workspace.element_size()
         if not workspace.is_contiguous():

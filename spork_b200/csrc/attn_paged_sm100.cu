@@ -5,14 +5,14 @@
 // products are small.  Work is cut along the cache: units of 64 keys (128 with a head dimension of 64: 32 KB of keys and
 // values) of one (request, key head), all units in one list, request by request, and each block of the grid takes an
 // equal run of that list, whatever the lengths (they are known on the device only).  A block joins what it computes of
-// one (request, key head) and writes the result if it has all of it; otherwise a partial result (running maximum, sum,
-// unnormalised output) goes to the workspace, and a second small kernel joins the parts in the order of the keys.  A
-// block has at most two partial results: its first run and its last one.
+// one (request, key head) and writes the result if it has all of it.  Otherwise it leaves a partial result (running
+// maximum, sum, unnormalised output) in the workspace and counts itself in; the block that comes last joins the parts,
+// eight at a time, in the order of the keys.  So one launch does, and what is added to what does not depend on who was last.
 //
 // One warp copies the pages with TMA: the cache is a 5-dimensional tensor (64 elements, page rows, halves of the head
 // dimension, heads, pages) with the strides that it has, so any order in memory is one tensor map; a box is a page's
 // rows of one head (64 rows of it at most), swizzled for ldmatrix.  Page numbers come from the block table, and are
-// checked before they are used.
+// checked before they are used.  With a unit goes a note that says what it is; only the copying warp walks the list.
 //
 // Four warps compute, each on keys of its own, with mma.m16n8k16.  Up to 8 query heads are rows 0-7 of the 16-row
 // operand, and rows 8-15 hold what rounding to 16 bits left over: of q, if it is fp32, and of the softmax weights.  So
@@ -50,11 +50,20 @@ constexpr float kShift = 6.0f, kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxBlocks = 1024;   // blocks of a launch
 constexpr int kComputeWarps = 4;
-constexpr int kThreads = (kComputeWarps + 1) * 32;
+// the computing warps, the copying one, and three idle ones that complete the second warpgroup, so that whole warpgroups
+// can trade registers
+constexpr int kThreads = 256;
 constexpr int kBlocksPerSm = 2;
+constexpr int kComputeRegs = 192, kCopyRegs = 64;
+// setmaxnreg.inc waits, without a limit, for registers to be free: the trade must fit what the block was launched with
+static_assert(kComputeRegs + kCopyRegs <= 2 * (65536 / (kThreads * kBlocksPerSm)), "register trade exceeds the launch allocation");
 constexpr int kPairCost = 1;       // what a (request, key head) costs a block besides its units, in units
+constexpr int kWhole = 4;          // a (request, key head) of so many units or fewer is not cut
+constexpr int kMinRun = 2;         // places of a block's run, at least
 constexpr int kMaxRows = 64;       // rows of a TMA box
-constexpr int kJoinThreads = 128;
+constexpr int kLengths = 512;      // requests whose lengths a block keeps in shared memory
+constexpr int kFan = 8;            // parts that are joined at a time
+constexpr int kLevels = 4;         // of joining: kFan^kLevels is more than the blocks of a launch
 
 // kGroups groups of warps share a unit, each with 8 query heads of its own.
 template <int D, int kGroups>
@@ -66,9 +75,9 @@ struct Config {
     static constexpr int kHalfUnit = kTile * D * 2;             // the keys (or values) of a unit, bytes
     static constexpr int kStageBytes = 2 * kHalfUnit;
     static constexpr int kStages = 3;
-    static constexpr int kPadded = D + 8;                       // floats between the rows of the joining buffer: no bank conflicts
-    static constexpr int kJoinFloats = kGroups * (kWarps - 1) * kHeads * kPadded;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kJoinFloats * 4;
+    static constexpr int kShare = D / 8 / kWarps;               // groups of 8 columns that a warp joins
+    static constexpr int kHanded = kHeads * kShare * 8;         // floats from one warp to another
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kComputeWarps * (kWarps - 1) * kHanded * 4;
 };
 
 struct Params {
@@ -79,73 +88,114 @@ struct Params {
     float* lse;
     int64_t q_request_stride, q_head_stride, table_stride;
     int32_t requests, heads, kv_heads, group, head_units;  // group: query heads per key head; head_units: units along them
-    int32_t max_blocks, num_pages, page_size, box_rows;
+    int32_t capacity;  // keys that a table row has room for (2^31 - 1 at most)
+    int32_t num_pages, page_size, box_rows;
     float scale_log2e;
     bool q_pairs;  // two neighbouring elements of q may be read at once
     // workspace
-    int4* joins;       // per block: {request (-1: none), key head and head unit, last block, slot of the first part}
-    float2* part_ml;   // [block][slot][head of the unit]: maximum, sum
-    float* part_o;     // [block][slot][head of the unit][D]
+    uint32_t* arrived; // [level][block][slot][warp]: parts that are there, of those whose first one is that; zero between calls
+    float2* part_ml;   // [block][slot][warp][head]: maximum, sum
+    float* part_o;     // [block][slot][warp][head][the warp's share of D]
     uint32_t* status;
 };
 
+// What a unit is.
+struct alignas(16) Note {
+    int r, kv, head;         // request, key head, first of the unit's query heads among those of the key head
+    int keys;                // keys that count from the unit's first one on (may be more than it has)
+    int position, count;     // which of the block's units of this (request, key head), and how many those are
+    int flags;               // bits as below
+    int parts, first;        // the blocks that have units of this (request, key head): how many, and the first one
+    int next_r, next_kv, next_head;  // with the last of the block's units: what comes next (-1: nothing)
+};
+// the run's end; this part is a later one of its block's (Walk::later); so is the first part; a bad page
+constexpr int kDone = 1, kLater = 2, kFirstLater = 4, kBad = 8;
+
 struct Bars {
-    uint64_t full[4];
-    uint64_t empty[4];
-    int64_t warp_sums[8];
-    int64_t start_base;    // the list's position of the block's first (request, head unit)
-    int32_t start[2];      // which one that is
-    int32_t bad[4];        // per stage: a page outside the cache
-    float2 ml[kComputeWarps][kHeads];
+    uint64_t full[4], empty[4];
+    uint64_t handed[kComputeWarps], taken[kComputeWarps];  // what others have for a warp is there; the warp has taken it
+    Note note[4];
+    uint32_t warp_sums[8];
+    uint32_t start[3];       // the block's first (request, head unit): request, which head unit, its place in the list
+    float2 ml[kComputeWarps][kComputeWarps][kHeads];  // [to][from]: maxima and sums
+    int32_t lengths[kLengths];  // of the first requests
     uint32_t abort_flag;
 };
-static_assert(2 * (Config<128, 1>::kSmem + (int)sizeof(Bars) + 1024) <= 228 * 1024, "two blocks to an SM");
+static_assert(kBlocksPerSm * (Config<128, 1>::kSmem + (int)sizeof(Bars) + 1024) <= 228 * 1024, "shared memory of the blocks of an SM");
 
 // Units of a request: none if there is nothing to read, or nothing that may be read.
 template <int kTile>
-__device__ __forceinline__ int units_of(const Params& p, int r)
+__device__ __forceinline__ int units_of(const Params& p, int len)
 {
-    const int64_t len = p.lengths[r];
-    return len > 0 && len <= (int64_t)p.max_blocks * p.page_size ? (int)((len + kTile - 1) / kTile) : 0;
+    return len > 0 && len <= p.capacity ? (int)(((uint32_t)len + kTile - 1) / kTile) : 0;
 }
 
+// The list cut into equal runs: block b's begins at place b * total / blocks.  (The host has made sure that a list has
+// fewer than 2^31 places.)
+struct Cut {
+    uint32_t total, blocks, each, rest;
+    __device__ __forceinline__ Cut(uint32_t places, uint32_t grid)
+        : total(places), blocks(places < grid * kMinRun ? (places + kMinRun - 1) / kMinRun : grid)
+    {
+        each = blocks ? total / blocks : 0;
+        rest = total - each * blocks;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t b) const { return b * each + b * rest / blocks; }
+    // the block whose run has a place
+    __device__ __forceinline__ uint32_t at(uint32_t place) const
+    {
+        return (uint32_t)(((uint64_t)(place + 1) * blocks - 1) / total);
+    }
+};
+
 // A block's run through the list, one (request, head unit) after the other.  Each takes its units' places in the list
-// and kPairCost more.
+// and kPairCost more.  One of kWhole units or fewer belongs to the block that has its middle unit's place.
 template <int kTile>
 struct Walk {
-    int r, hh, first, count, units, len;
-    int64_t base, end;  // places in the list: of the current one's first unit, of the end of the run
-    bool any;           // whether the block has had units before the current ones
+    int r, kv, hu, first, count, units, len;
+    uint32_t base, from, end;  // places in the list: of the current one's first unit, of the run's begin and end
 
-    __device__ __forceinline__ void here(const Params& p, int64_t from)
+    __device__ __forceinline__ void here()
     {
-        len = p.lengths[r];
-        units = (int)(((int64_t)len + kTile - 1) / kTile);
-        first = from > base ? (int)(from - base) : 0;
-        const int64_t last = end - base < units ? end - base : units;
-        count = last > first ? (int)(last - first) : 0;
+        if (units <= kWhole) {
+            const uint32_t middle = base + units / 2;
+            first = 0;
+            count = middle >= from && middle < end ? units : 0;
+        } else {
+            first = from > base ? (int)(from - base) : 0;
+            const int last = (int)(end - base) < units ? (int)(end - base) : units;
+            count = last > first ? last - first : 0;
+        }
     }
     // to the next one; false at the run's end
-    __device__ __forceinline__ bool next(const Params& p)
+    template <typename Length>
+    __device__ __forceinline__ bool next(const Params& p, const Length& length)
     {
-        any = any || count > 0;
         base += units + kPairCost;
         if (base >= end) {
             return false;
         }
-        if (++hh == p.kv_heads * p.head_units) {
-            hh = 0;
-            do {
-                ++r;
-                if (r >= p.requests) {
-                    return false;
-                }
-            } while (units_of<kTile>(p, r) == 0);
+        if (++hu == p.head_units) {
+            hu = 0;
+            if (++kv == p.kv_heads) {
+                kv = 0;
+                do {
+                    if (++r >= p.requests) {
+                        return false;
+                    }
+                    len = length(r);
+                    units = units_of<kTile>(p, len);
+                } while (units == 0);
+            }
         }
-        here(p, base);
+        here();
         return true;
     }
 };
+
+// Where a block's part of a (request, head unit) goes in the workspace: a run that begins in front of it (and of its
+// predecessor's cost) has other units first, and at its begin it may have a part of those.
+__device__ __forceinline__ bool is_later(uint32_t from, uint32_t base) { return from + kPairCost < base; }
 
 __device__ __forceinline__ float ex2(float x)
 {
@@ -193,42 +243,58 @@ __device__ __forceinline__ void report_timeout(const Params& p, volatile uint32_
     atomicCAS(p.status, 0u, 0x90000000u | (role << 24) | ((where & 0xFFu) << 16) | (blockIdx.x & 0xFFFFu));
 }
 
-// Two neighbouring elements of q as 32-bit numbers; `pairs`: they may be read at once.
-template <typename Q>
-__device__ __forceinline__ float2 load_two(const Q* q, bool pairs)
+// Two neighbouring elements of q; `pairs`: they may be read at once.
+__device__ __forceinline__ float2 load_two(const float* q, bool pairs)
 {
-    if (pairs) {
-        if constexpr (std::is_same<Q, float>::value) {
-            return *reinterpret_cast<const float2*>(q);
-        } else {
-            return unpack<Q>(*reinterpret_cast<const uint32_t*>(q));
-        }
-    }
-    return make_float2(to_f32(q[0]), to_f32(q[1]));
+    return pairs ? *reinterpret_cast<const float2*>(q) : make_float2(q[0], q[1]);
 }
-
-// Asks for the line of an address in L1 without waiting for it.
-__device__ __forceinline__ void touch(const void* p)
+__device__ __forceinline__ uint32_t load_two(const void* q, bool pairs)
 {
-    asm volatile(
-        "{\n\t"
-        ".reg .u16 unused;\n\t"
-        "ld.global.ca.u16 unused, [%0];\n\t"
-        "}" ::"l"(p));
+    const uint16_t* x = static_cast<const uint16_t*>(q);
+    return pairs ? *reinterpret_cast<const uint32_t*>(q) : x[0] | (uint32_t)x[1] << 16;
 }
 
 // What one warp has of its 8 query heads and a run of keys: maxima, sums, unnormalised output (fragments: row g of the
-// first product's operand is in [0], [1], row g + 8, its low part, in [2], [3]).
-template <int D, typename T, bool kLowQ, int kChunk>
+// first product's operand is in [0], [1], row g + 8, its low part, in [2], [3]); and the weights of the unit at hand.
+template <int D, typename T, bool kLowQ, int kKeys>
 struct Softmax {
     static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-    static constexpr int kSteps = D / 16, kPairs = kChunk / 16;
+    static constexpr int kSteps = D / 16, kPairs = kKeys / 16;
     uint32_t q_hi[kSteps][2], q_lo[kLowQ ? kSteps : 1][2];
     float acc[D / 8][4];
     float m, l;  // of row g; l: this lane's columns only
+    uint32_t weights[kPairs][4];
 
-    __device__ __forceinline__ void clear()
+    // The queries as they are (kLowQ: 32 bits), on their way into the registers that begin() makes operands of.
+    template <typename Q>
+    __device__ __forceinline__ void ask_for(const Q* q, bool here, bool pairs)
     {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if constexpr (kLowQ) {
+                    const float2 x = here ? load_two(q + i * 16 + j * 8, pairs) : make_float2(0.0f, 0.0f);
+                    q_hi[i][j] = __float_as_uint(x.x);
+                    q_lo[i][j] = __float_as_uint(x.y);
+                } else {
+                    q_hi[i][j] = here ? load_two(q + i * 16 + j * 8, pairs) : 0u;
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void begin()
+    {
+        if constexpr (kLowQ) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    split<T>(__uint_as_float(q_hi[i][j]), __uint_as_float(q_lo[i][j]), q_hi[i][j], q_lo[i][j]);
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
             acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
@@ -237,11 +303,10 @@ struct Softmax {
         l = 0.0f;
     }
 
-    // kChunk keys, whose rows for ldmatrix are at k_row and v_row; `keys` of them count (kRagged: not all, and the rest
+    // Weights of a unit's keys, whose rows for ldmatrix are at `row`; `keys` of them count (kRagged: not all, and the rest
     // may be anything).
     template <bool kRagged>
-    __device__ __forceinline__ void add(const uint32_t (&k_row)[kPairs], const uint32_t (&v_row)[kPairs], uint32_t half,
-                                        int keys, float scale)
+    __device__ __forceinline__ void take_keys(const uint32_t (&row)[kPairs], uint32_t base, uint32_t half, int keys, float scale)
     {
         const int lane = threadIdx.x % 32, t = lane % 4, matrix = lane / 8, row8 = lane % 8;
         float s[2 * kPairs][4];
@@ -253,11 +318,13 @@ struct Softmax {
         for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
             for (int n = 0; n < kPairs; ++n) {
-                uint32_t b[4];
-                ldmatrix_x4(k_row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix % 2) ^ row8) << 4), b);
-                const uint32_t a1 = kLowQ ? q_lo[kLowQ ? i : 0][0] : 0u, a3 = kLowQ ? q_lo[kLowQ ? i : 0][1] : 0u;
-                mma_m16n8k16<kBf16>(s[2 * n], q_hi[i][0], a1, q_hi[i][1], a3, b[0], b[1]);
-                mma_m16n8k16<kBf16>(s[2 * n + 1], q_hi[i][0], a1, q_hi[i][1], a3, b[2], b[3]);
+                if (!kRagged || n * 16 < keys) {
+                    uint32_t b[4];
+                    ldmatrix_x4(base + row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix % 2) ^ row8) << 4), b);
+                    const uint32_t a1 = kLowQ ? q_lo[kLowQ ? i : 0][0] : 0u, a3 = kLowQ ? q_lo[kLowQ ? i : 0][1] : 0u;
+                    mma_m16n8k16<kBf16>(s[2 * n], q_hi[i][0], a1, q_hi[i][1], a3, b[0], b[1]);
+                    mma_m16n8k16<kBf16>(s[2 * n + 1], q_hi[i][0], a1, q_hi[i][1], a3, b[2], b[3]);
+                }
             }
         }
         float most = -INFINITY;
@@ -297,14 +364,27 @@ struct Softmax {
 #pragma unroll
         for (int n = 0; n < kPairs; ++n) {
             float w[4];
-            uint32_t a[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 w[j] = ex2(fmaf(s[2 * n + j / 2][j % 2], scale, shift));
                 l += w[j];
             }
-            split<T>(w[0], w[1], a[0], a[1]);
-            split<T>(w[2], w[3], a[2], a[3]);
+            split<T>(w[0], w[1], weights[n][0], weights[n][1]);
+            split<T>(w[2], w[3], weights[n][2], weights[n][3]);
+        }
+    }
+
+    // The same unit's values.
+    template <bool kRagged>
+    __device__ __forceinline__ void take_values(const uint32_t (&row)[kPairs], uint32_t base, uint32_t half, int keys)
+    {
+        const int lane = threadIdx.x % 32, t = lane % 4, matrix = lane / 8, row8 = lane % 8;
+#pragma unroll
+        for (int n = 0; n < kPairs; ++n) {
+            if (kRagged && n * 16 >= keys) {
+                continue;
+            }
+            const uint32_t(&a)[4] = weights[n];
             // a value that does not count may be NaN, and its weight of zero would not remove it
             uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
             if (kRagged) {
@@ -315,7 +395,7 @@ struct Softmax {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 uint32_t b[4];
-                ldmatrix_x4_trans(v_row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix / 2) ^ row8) << 4), b);
+                ldmatrix_x4_trans(base + row[n] + (i / 4) * half + ((((i % 4) * 2 + matrix / 2) ^ row8) << 4), b);
                 mma_m16n8k16<kBf16>(acc[2 * i], a[0], a[1], a[2], a[3], kRagged ? b[0] & keep0 : b[0],
                                     kRagged ? b[1] & keep1 : b[1]);
                 mma_m16n8k16<kBf16>(acc[2 * i + 1], a[0], a[1], a[2], a[3], kRagged ? b[2] & keep0 : b[2],
@@ -325,26 +405,150 @@ struct Softmax {
     }
 };
 
+// A warp's share of a result: lane (g, t) has row g's columns 8 i + 2 t and + 1 of it, and the row's maximum and sum.
+template <int kShare>
+struct Part {
+    float2 o[kShare];
+    float m, l;
+
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int i = 0; i < kShare; ++i) {
+            o[i] = make_float2(0.0f, 0.0f);
+        }
+        m = -INFINITY;
+        l = 0.0f;
+    }
+
+    __device__ __forceinline__ void join(float its_m, float its_l, const float2 (&its_o)[kShare])
+    {
+        const float most = fmaxf(m, its_m), to = most == -INFINITY ? 0.0f : most;
+        const float down = ex2(m - to), its_down = ex2(its_m - to);
+        l = l * down + its_l * its_down;
+        m = most;
+#pragma unroll
+        for (int i = 0; i < kShare; ++i) {
+            o[i].x = o[i].x * down + its_o[i].x * its_down;
+            o[i].y = o[i].y * down + its_o[i].y * its_down;
+        }
+    }
+};
+
+// Row `row` of the output: the share's columns from `column` on.
+template <typename T, int D, int kShare>
+__device__ __forceinline__ void write_result(const Params& p, const Part<kShare>& all, int64_t row, int column)
+{
+    const int t = threadIdx.x % 4;
+    const float by = 1.0f / all.l;
+    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + row * D + column) + t;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+        out[i * 4] = pack<T>(all.o[i].x * by, all.o[i].y * by);
+    }
+    if (p.lse && t == 0 && column == 0) {
+        p.lse[row] = ((all.m == -INFINITY ? 0.0f : all.m) - kShift + log2f(all.l)) * kLn2;
+    }
+}
+
+template <int kShare>
+__device__ __forceinline__ void write_part(const Params& p, const Part<kShare>& all, int64_t row)
+{
+    const int t = threadIdx.x % 4;
+    float* out = p.part_o + row * (kShare * 8) + 2 * t;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+        __stcg(reinterpret_cast<float2*>(out + i * 8), all.o[i]);
+    }
+    if (t == 0) {
+        __stcg(p.part_ml + row, make_float2(all.m, all.l));
+    }
+}
+
+// A warp writes its share of this block's part, and counts it in.  The parts are those of blocks first .. first + parts - 1
+// (the first one in that block's slot first_slot, the others in slot 0).  The last of every kFan joins these in order and
+// leaves the result where the first of them was, and so on; the last of all returns true with the whole.
+template <int kShare>
+__device__ __forceinline__ bool join_parts(const Params& p, Part<kShare>& all, int warp, int first, int parts, int first_slot)
+{
+    const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    auto place = [&](int i) { return ((int64_t)(first + i) * 2 + (i == 0 ? first_slot : 0)) * kComputeWarps + warp; };
+    auto row_of = [&](int i) { return place(i) * kHeads + g; };
+    int mine = (int)blockIdx.x - first, step = 1;  // part i of a level is where part i * step of the lowest one was
+    bool written = false;
+    for (int n = parts, level = 0; n > 1; n = (n + kFan - 1) / kFan, ++level, step *= kFan, mine /= kFan) {
+        if (!written) {
+            write_part(p, all, row_of(mine * step));
+            written = true;
+        }
+        const int begin = mine / kFan * kFan, members = n - begin < kFan ? n - begin : kFan;
+        if (members == 1) {
+            continue;  // it is its own join, where it is
+        }
+        uint32_t* counter = p.arrived + (int64_t)level * gridDim.x * 2 * kComputeWarps + place(begin * step);
+        __syncwarp();
+        uint32_t before = 0;
+        if (lane == 0) {
+            // releases what the warp has written, and acquires what the others had when they counted themselves in
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+        }
+        before = __shfl_sync(0xFFFFFFFFu, before, 0);
+        __syncwarp();
+        if (before != (uint32_t)members - 1u) {
+            return false;
+        }
+        if (lane == 0) {
+            *counter = 0u;  // for the next launch
+        }
+        all.clear();
+        constexpr int kAtOnce = kShare <= 4 ? 4 : kShare == 8 ? 2 : 1;
+        for (int k = 0; k < members; k += kAtOnce) {
+            float2 ml[kAtOnce], o[kAtOnce][kShare];
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+                if (x == 0 || k + x < members) {
+                    const int64_t from = row_of((begin + k + x) * step);
+                    ml[x] = __ldcg(p.part_ml + from);
+#pragma unroll
+                    for (int i = 0; i < kShare; ++i) {
+                        o[x][i] = __ldcg(reinterpret_cast<const float2*>(p.part_o + from * (kShare * 8) + 2 * t + i * 8));
+                    }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+                if (x == 0 || k + x < members) {
+                    all.join(ml[x].x, ml[x].y, o[x]);
+                }
+            }
+        }
+        written = false;
+    }
+    return true;
+}
+
 template <int D, typename T, typename Q, int kGroups>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     attn_paged_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p)
 {
     using Cfg = Config<D, kGroups>;
-    using W = Walk<Cfg::kTile>;
     constexpr bool kLowQ = std::is_same<Q, float>::value;  // q has a low part
     constexpr int kUnitHeads = kGroups * kHeads;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Bars bars;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    float* join = reinterpret_cast<float*>(smem_raw + (stages - smem_u32(smem_raw)) + Cfg::kStages * Cfg::kStageBytes);
+    float* handed = reinterpret_cast<float*>(smem_raw + (stages - smem_u32(smem_raw)) + Cfg::kStages * Cfg::kStageBytes);
     volatile uint32_t* abort_flag = &bars.abort_flag;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(smem_u32(&bars.full[s]), 1);
             mbar_init(smem_u32(&bars.empty[s]), kComputeWarps);
-            bars.bad[s] = 0;
+        }
+        for (int w = 0; w < kComputeWarps; ++w) {
+            mbar_init(smem_u32(&bars.handed[w]), Cfg::kWarps > 1 ? Cfg::kWarps - 1 : 1);
+            mbar_init(smem_u32(&bars.taken[w]), 1);
         }
         bars.abort_flag = 0;
         fence_mbar_init();
@@ -359,123 +563,141 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 
     // ------------------------------------------------------------ this block's run of the list
     const int hhs = p.kv_heads * p.head_units;
-    int64_t total = 0;  // places in the list
-    {
-        const int chunk = (p.requests + kThreads - 1) / kThreads;
-        const int r0 = (int)threadIdx.x * chunk, r1 = r0 + chunk < p.requests ? r0 + chunk : p.requests;
-        const auto places = [&](int r) {
-            const int units = units_of<Cfg::kTile>(p, r);
-            return units ? (int64_t)(units + kPairCost) * hhs : 0;
-        };
-        int64_t mine = 0;
-        for (int r = r0; r < r1; ++r) {
-            mine += places(r);
+    const int chunk = (p.requests + kThreads - 1) / kThreads;
+    const int r0 = (int)threadIdx.x * chunk, r1 = r0 + chunk < p.requests ? r0 + chunk : p.requests;
+    const auto places_of = [&](int len) {
+        const int units = units_of<Cfg::kTile>(p, len);
+        return units ? (uint32_t)(units + kPairCost) * hhs : 0u;
+    };
+    uint32_t mine = 0;  // places of this thread's requests
+    for (int r = r0; r < r1; ++r) {
+        const int len = p.lengths[r];
+        if (r < kLengths) {
+            bars.lengths[r] = len;
         }
-        int64_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int64_t w = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-            upto += lane >= d ? w : 0;
-        }
-        if (lane == 31) {
-            bars.warp_sums[warp] = upto;
-        }
-        __syncthreads();
-        int64_t base = upto - mine;
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) {
-            base += w < warp ? bars.warp_sums[w] : 0;
-            total += bars.warp_sums[w];
-        }
-        const int64_t blocks = total < gridDim.x ? total : gridDim.x;
-        if (blockIdx.x < blocks) {
-            const int64_t u0 = blockIdx.x * total / blocks;
-            if (u0 >= base && u0 < base + mine) {
-                int r = r0;
-                int64_t its = places(r);
-                while (u0 >= base + its) {
-                    base += its;
-                    its = places(++r);
-                }
-                const int hh = (int)((u0 - base) / (its / hhs));
-                bars.start[0] = r;
-                bars.start[1] = hh;
-                bars.start_base = base + hh * (its / hhs);
-            }
-        }
-        __syncthreads();
+        mine += places_of(len);
     }
-    const int64_t blocks = total < gridDim.x ? total : gridDim.x;
-    const bool work = blockIdx.x < blocks;
-    W walk{};
+    const auto length = [&](int r) { return r < kLengths ? bars.lengths[r] : p.lengths[r]; };
+    uint32_t base = mine, places = 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t w = __shfl_up_sync(0xFFFFFFFFu, base, d);
+        base += lane >= d ? w : 0;
+    }
+    if (lane == 31) {
+        bars.warp_sums[warp] = base;
+    }
+    __syncthreads();
+    base -= mine;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        base += w < warp ? bars.warp_sums[w] : 0;
+        places += bars.warp_sums[w];
+    }
+    const Cut cut(places, gridDim.x);
+    const bool work = blockIdx.x < cut.blocks;
+    const uint32_t from = work ? cut.begin(blockIdx.x) : 0;
+    if (work && from - base < mine) {
+        int r = r0;
+        uint32_t its = places_of(length(r));
+        while (from - base >= its) {
+            base += its;
+            its = places_of(length(++r));
+        }
+        const uint32_t each = its / hhs, hh = (from - base) / each;
+        bars.start[0] = r;
+        bars.start[1] = hh;
+        bars.start[2] = base + hh * each;
+    }
+    __syncthreads();
+    Walk<Cfg::kTile> walk{};
     if (work) {
         walk.r = bars.start[0];
-        walk.hh = bars.start[1];
-        walk.base = bars.start_base;
-        walk.end = (blockIdx.x + 1) * total / blocks;
-        walk.here(p, blockIdx.x * total / blocks);
+        walk.kv = p.head_units == 1 ? bars.start[1] : bars.start[1] / p.head_units;
+        walk.hu = bars.start[1] - walk.kv * p.head_units;
+        walk.base = bars.start[2];
+        walk.from = from;
+        walk.end = cut.begin(blockIdx.x + 1);
+        walk.len = length(walk.r);
+        walk.units = units_of<Cfg::kTile>(p, walk.len);
+        walk.here();
     }
-    if (threadIdx.x == 0) {
-        // The first block whose run begins after the first unit of a (request, head unit), and before its end, names the
-        // parts of it: the block before has the first one (as its first run of units or a later one), then this block and
-        // those behind it as their first.
-        int4 j = make_int4(-1, 0, 0, 0);
-        if (work && walk.first > 0 && walk.count > 0) {
-            const int64_t previous = (blockIdx.x - 1) * total / blocks;
-            if (previous <= walk.base) {
-                const int64_t last = walk.base + walk.units - 1;
-                j = make_int4(walk.r, walk.hh, (int)(((last + 1) * blocks - 1) / total),
-                              previous >= walk.base - kPairCost ? 0 : 1);
-            }
+    // to the first (request, head unit) from here on that has units for this block
+    auto settle = [&](bool more) {
+        while (more && walk.count == 0) {
+            more = walk.next(p, length);
         }
-        p.joins[blockIdx.x] = j;
-    }
+        return more;
+    };
+    bool more = settle(work);
 
     const int rows = p.box_rows;
-    if (warp == kComputeWarps) {
+    if (warp >= kComputeWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegs));
+        if (warp > kComputeWarps) {
+            return;
+        }
         // -------------------------------------------------------------------------------------- copies
         const Checker ck{p.status, stages, stages + Cfg::kStages * Cfg::kStageBytes, 0, 0};
         const int boxes = Cfg::kTile / rows;
         const uint32_t box_bytes = rows * D * 2;
         uint32_t stage = 0, phase = 0, used = 0;
         bool ok = true;
-        // to the first (request, head unit) from here on that has units for this block
-        auto settle = [&](bool more) {
-            while (more && walk.count == 0) {
-                more = walk.next(p);
-            }
-            return more;
-        };
-        bool more = settle(work);
         int unit = walk.first;
-        // the page of this lane's box of a unit; -1 if it is behind the last key
-        auto page_of = [&](int u) {
-            const int64_t at = (int64_t)u * Cfg::kTile + lane * rows;
-            return lane < boxes && at < walk.len ? p.table[walk.r * p.table_stride + (uint32_t)at / (uint32_t)p.page_size] : -1;
+        // A unit with its note, and this lane's box of it: its page and its first row there.
+        struct Plan {
+            Note note;
+            int page, row;
+            bool mine;
         };
-        int page = more ? page_of(unit) : -1;
-        while (more) {
-            const int64_t at = (int64_t)unit * Cfg::kTile + lane * rows;
-            const bool mine = lane < boxes && at < walk.len;
-            const int this_page = page, head = walk.hh / p.head_units;
-            const int row = mine ? (int)((uint32_t)at % (uint32_t)p.page_size) : 0;
+        auto look_ahead = [&] {
+            Plan plan;
+            plan.page = plan.row = 0;
+            plan.mine = false;
+            plan.note.next_r = -1;
+            plan.note.next_kv = plan.note.next_head = 0;
+            plan.note.flags = kDone;
+            if (!more) {
+                return plan;
+            }
+            const int first = unit * Cfg::kTile, keys = walk.len - first;
+            if (lane < boxes && lane * rows < keys) {
+                const uint32_t at = (uint32_t)(first + lane * rows), block = at / (uint32_t)p.page_size;
+                plan.mine = true;
+                plan.row = (int)(at - block * (uint32_t)p.page_size);
+                plan.page = p.table[walk.r * p.table_stride + block];
+            }
+            plan.note.r = walk.r;
+            plan.note.kv = walk.kv;
+            plan.note.head = walk.hu * kUnitHeads;
+            plan.note.keys = keys;
+            plan.note.position = unit - walk.first;
+            plan.note.count = walk.count;
+            plan.note.flags = 0;
+            plan.note.parts = 1;
+            plan.note.first = 0;
             if (++unit == walk.first + walk.count) {
-                more = settle(walk.next(p));
+                if (walk.count != walk.units) {
+                    const uint32_t first_block = cut.at(walk.base);
+                    plan.note.first = (int)first_block;
+                    plan.note.parts = (int)(cut.at(walk.base + walk.units - 1) - first_block) + 1;
+                    plan.note.flags = (is_later(from, walk.base) ? kLater : 0) |
+                                      (is_later(cut.begin(first_block), walk.base) ? kFirstLater : 0);
+                }
+                more = settle(walk.next(p, length));
                 unit = walk.first;
                 if (more) {
-                    // the queries of what comes next, on their way while the units before it are worked on: a line per lane
-                    constexpr int kLines = D * (int)sizeof(Q) / 128;
-                    for (int i = lane; i < kUnitHeads * kLines; i += 32) {
-                        const int in_group = (walk.hh % p.head_units) * kUnitHeads + i / kLines;
-                        if (in_group < p.group) {
-                            touch(static_cast<const Q*>(p.q) + walk.r * p.q_request_stride +
-                                  (int64_t)(walk.hh / p.head_units * p.group + in_group) * p.q_head_stride +
-                                  (i % kLines) * (128 / (int)sizeof(Q)));
-                        }
-                    }
+                    plan.note.next_r = walk.r;
+                    plan.note.next_kv = walk.kv;
+                    plan.note.next_head = walk.hu * kUnitHeads;
                 }
             }
-            page = more ? page_of(unit) : -1;  // asked for one unit ahead
+            return plan;
+        };
+        // the run's units, then a note of its end; a page is asked for while the two units before its own are copied
+        Plan plan = look_ahead(), next = look_ahead();
+        while (true) {
+            const bool end = plan.note.flags & kDone;
             ok = mbar_wait(smem_u32(&bars.empty[stage]), phase ^ 1u, abort_flag);
             if (!ok && lane == 0) {
                 report_timeout(p, abort_flag, 1, stage);
@@ -484,25 +706,31 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             if (!ok) {
                 break;
             }
-            const bool good = mine && this_page >= 0 && this_page < p.num_pages;
-            const uint32_t bad = __ballot_sync(0xFFFFFFFFu, mine && !good), valid = __ballot_sync(0xFFFFFFFFu, good);
+            const bool good = plan.mine && plan.page >= 0 && plan.page < p.num_pages;
+            const uint32_t bad = __ballot_sync(0xFFFFFFFFu, plan.mine && !good), valid = __ballot_sync(0xFFFFFFFFu, good);
             const uint32_t full = smem_u32(&bars.full[stage]);
             const uint32_t keys = stages + stage * Cfg::kStageBytes + lane * box_bytes;
             if (lane == 0) {
-                bars.bad[stage] = bad != 0;
+                plan.note.flags |= bad ? kBad : 0;
+                bars.note[stage] = plan.note;
                 mbar_arrive_expect_tx(full, 2 * box_bytes * __popc(valid));
             }
             __syncwarp();
             if (good && ck.smem(keys, box_bytes, 1024, 0x501) && ck.smem(keys + Cfg::kHalfUnit, box_bytes, 1024, 0x502) &&
-                ck.tma_coords(0, 2, row, this_page, 0x503)) {
-                tma_load_5d(keys, &map_k, full, 0, row, 0, head, this_page);
-                tma_load_5d(keys + Cfg::kHalfUnit, &map_v, full, 0, row, 0, head, this_page);
+                ck.tma_coords(0, 2, plan.row, plan.page, 0x503)) {
+                tma_load_5d(keys, &map_k, full, 0, plan.row, 0, plan.note.kv, plan.page);
+                tma_load_5d(keys + Cfg::kHalfUnit, &map_v, full, 0, plan.row, 0, plan.note.kv, plan.page);
             }
             ++used;
+            if (end) {
+                break;
+            }
             if (++stage == Cfg::kStages) {
                 stage = 0;
                 phase ^= 1u;
             }
+            plan = next;
+            next = look_ahead();
         }
         if (!ok) {
             // copies that are still under way end before the block does (each wait has its limit)
@@ -516,268 +744,176 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         }
     } else {
         // ------------------------------------------------------------------------------------- products
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
         const int group = warp / Cfg::kWarps, part = warp % Cfg::kWarps;  // group of warps, warp of the group
         const int g = lane / 4, t = lane % 4;                             // row (query head) and column pair of a fragment
         const int matrix = lane / 8, row8 = lane % 8;
         using S = Softmax<D, T, kLowQ, Cfg::kChunk>;
-        constexpr int kPairs = S::kPairs, kSteps = S::kSteps, kChunks = Cfg::kKeys / Cfg::kChunk;
-        // shared-memory offsets of this lane's ldmatrix rows: keys (matrices 0, 1 | 2, 3 are keys 0-7 | 8-15) and values
+        constexpr int kPairs = S::kPairs, kChunks = Cfg::kKeys / Cfg::kChunk;
+        S sm;
+        auto ask_for = [&](int r, int kv, int head) {
+            const int in_group = head + group * kHeads + g;
+            const bool here = in_group < p.group;
+            sm.ask_for(static_cast<const Q*>(p.q) + r * p.q_request_stride +
+                           (int64_t)(kv * p.group + (here ? in_group : 0)) * p.q_head_stride + 2 * t,
+                       here, p.q_pairs);
+        };
+        if (more) {
+            ask_for(walk.r, walk.kv, walk.hu * kUnitHeads);
+        }
+        // offsets in a stage of this lane's ldmatrix rows: keys (matrices 0, 1 | 2, 3 are keys 0-7 | 8-15) and values
         // (matrices 0, 2 | 1, 3); a box of `rows` rows holds its halves of 64 columns one behind the other
         auto row_at = [&](int r) { return (uint32_t)((r / rows) * rows * D * 2 + (r % rows) * 128); };
-        uint32_t k_at[kChunks][kPairs], v_at[kChunks][kPairs];
+        uint32_t k_row[kChunks][kPairs], v_row[kChunks][kPairs];
         for (int c = 0; c < kChunks; ++c) {
             for (int i = 0; i < kPairs; ++i) {
                 const int r = part * Cfg::kKeys + c * Cfg::kChunk + i * 16 + row8;
-                k_at[c][i] = row_at(r + (matrix / 2) * 8);
-                v_at[c][i] = row_at(r + (matrix % 2) * 8) + Cfg::kHalfUnit;
+                k_row[c][i] = row_at(r + (matrix / 2) * 8);
+                v_row[c][i] = row_at(r + (matrix % 2) * 8) + Cfg::kHalfUnit;
             }
         }
         const uint32_t half = rows * 128;
-        uint32_t stage = 0, phase = 0;
-        bool ok = true, joined = false;
-        S sm;
+        uint32_t stage = 0, phase = 0, times = 0;  // times: that sums have been handed over
+        bool ok = true;
+        int bad = 0;
+        // every lane polls; false if the wait was given up
+        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t role, uint32_t where) {
+            const bool done = mbar_wait(smem_u32(bar), parity, abort_flag);
+            if (!done) {
+                report_timeout(p, abort_flag, role, where);
+            }
+            return __all_sync(0xFFFFFFFFu, done);
+        };
 
-        for (bool more = work; more; more = walk.next(p)) {
-            if (walk.count == 0) {
+        while (true) {
+            ok = wait(&bars.full[stage], phase, 2, stage);
+            const Note& note = bars.note[stage];
+            const int4 what = *reinterpret_cast<const int4*>(&note.r), which = *reinterpret_cast<const int4*>(&note.position);
+            const int4 next = *reinterpret_cast<const int4*>(&note.first);  // first block of the parts; what comes next
+            const int left = what.w - part * Cfg::kKeys, flags = which.z;
+            if (!ok || (flags & kDone)) {
+                break;
+            }
+            if (which.x == 0) {
+                sm.begin();
+                bad = 0;
+            }
+            bad |= flags & kBad;
+            const bool last = which.x + 1 == which.y;
+            const uint32_t memory = stages + stage * Cfg::kStageBytes;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int keys = left - c * Cfg::kChunk;
+                if (keys >= Cfg::kChunk) {
+                    sm.template take_keys<false>(k_row[c], memory, half, keys, p.scale_log2e);
+                } else if (keys > 0) {
+                    sm.template take_keys<true>(k_row[c], memory, half, keys, p.scale_log2e);
+                }
+                if (c == kChunks - 1 && last && next.y >= 0) {
+                    // the old queries have done their work: the next ones arrive while the values are worked on
+                    ask_for(next.y, next.z, next.w);
+                }
+                if (keys >= Cfg::kChunk) {
+                    sm.template take_values<false>(v_row[c], memory, half, keys);
+                } else if (keys > 0) {
+                    sm.template take_values<true>(v_row[c], memory, half, keys);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&bars.empty[stage]));
+            }
+            if (++stage == Cfg::kStages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+            if (!last) {
                 continue;
             }
-            const int kv = walk.hh / p.head_units, in_group = (walk.hh % p.head_units) * kUnitHeads + group * kHeads + g;
-            const bool head_here = in_group < p.group;
-            // q: rows g and, for what rounding left over, g + 8 of the A operand
-            {
-                const Q* q = static_cast<const Q*>(p.q) + walk.r * p.q_request_stride +
-                             (int64_t)(kv * p.group + (head_here ? in_group : 0)) * p.q_head_stride + 2 * t;
+
+            // ------------------------------------------------- the warps of the group joined, the result or part written
+            // Each warp hands every other one of its group that one's share of the columns, and joins its own.
+            float l = sm.l + __shfl_xor_sync(0xFFFFFFFFu, sm.l, 1);
+            l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+            l = bad ? NAN : l;
+            constexpr int kWarps = Cfg::kWarps, kShare = Cfg::kShare;
+            // groups of 8 columns change places by row, so that no two rows' meet in a bank
+            auto turned = [&](int i) { return i ^ ((kShare == 2 ? g >> 1 : g) & (kShare - 1)); };
+            Part<kShare> all;
+            all.m = sm.m;
+            all.l = l;
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
+            for (int w = 0; w < kWarps; ++w) {
+                const int to = group * kWarps + w;
+                if (w == part) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float2 x = load_two(q + i * 16 + j * 8, p.q_pairs);
-                        x = head_here ? x : make_float2(0.0f, 0.0f);
-                        if (kLowQ) {
-                            split<T>(x.x, x.y, sm.q_hi[i][j], sm.q_lo[kLowQ ? i : 0][j]);
-                        } else {
-                            sm.q_hi[i][j] = pack<T>(x.x, x.y);
+                    for (int i = 0; i < kShare; ++i) {
+                        const float(&a)[4] = sm.acc[w * kShare + i];
+                        all.o[i] = make_float2(a[0] + a[2], a[1] + a[3]);
+                    }
+                } else {
+                    ok = ok && wait(&bars.taken[to], (times & 1u) ^ 1u, 3, to);
+                    if (ok) {
+                        float* row = handed + (to * (kWarps - 1) + (part < w ? part : part - 1)) * Cfg::kHanded + g * kShare * 8 + 2 * t;
+#pragma unroll
+                        for (int i = 0; i < kShare; ++i) {
+                            const float(&a)[4] = sm.acc[w * kShare + i];
+                            *reinterpret_cast<float2*>(row + turned(i) * 8) = make_float2(a[0] + a[2], a[1] + a[3]);
+                        }
+                        if (t == 0) {
+                            bars.ml[to][warp][g] = make_float2(sm.m, l);
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(smem_u32(&bars.handed[to]));
                         }
                     }
                 }
             }
-            sm.clear();
-            int bad = 0;
-
-            for (int u = walk.first; u < walk.first + walk.count; ++u) {
-                if (ok && !mbar_wait(smem_u32(&bars.full[stage]), phase, abort_flag)) {
-                    report_timeout(p, abort_flag, 2, stage);
-                    ok = false;
-                }
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                bad |= *const_cast<volatile int32_t*>(&bars.bad[stage]);
-                const uint32_t base = stages + stage * Cfg::kStageBytes;
-                const int64_t left = walk.len - (int64_t)u * Cfg::kTile - part * Cfg::kKeys;  // keys from this warp's first on
+            if (kWarps > 1) {
+                ok = ok && wait(&bars.handed[warp], times & 1u, 4, warp);
+                if (ok) {
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    uint32_t k_row[kPairs], v_row[kPairs];
+                    for (int w = 0; w < kWarps - 1; ++w) {
+                        const float* row = handed + (warp * (kWarps - 1) + w) * Cfg::kHanded + g * kShare * 8 + 2 * t;
+                        const float2 ml = bars.ml[warp][group * kWarps + (w < part ? w : w + 1)][g];
+                        float2 o[kShare];
 #pragma unroll
-                    for (int i = 0; i < kPairs; ++i) {
-                        k_row[i] = base + k_at[c][i];
-                        v_row[i] = base + v_at[c][i];
+                        for (int i = 0; i < kShare; ++i) {
+                            o[i] = *reinterpret_cast<const float2*>(row + turned(i) * 8);
+                        }
+                        all.join(ml.x, ml.y, o);
                     }
-                    const int keys = left > Cfg::kTile ? Cfg::kTile : (int)left - c * Cfg::kChunk;
-                    if (ok && keys >= Cfg::kChunk) {
-                        sm.template add<false>(k_row, v_row, half, keys, p.scale_log2e);
-                    } else if (ok && keys > 0) {
-                        sm.template add<true>(k_row, v_row, half, keys, p.scale_log2e);
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&bars.taken[warp]));
                     }
                 }
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&bars.empty[stage]));
-                }
-                if (++stage == Cfg::kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
+                ++times;
             }
-
-            // ------------------------------------------------- the warps of the group joined, the result or part written
-            float o[D / 8][2], m = sm.m, l = sm.l;
-            l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-            l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-            l = bad ? NAN : l;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] = sm.acc[i][0] + sm.acc[i][2];
-                o[i][1] = sm.acc[i][1] + sm.acc[i][3];
+            if (!ok) {
+                break;
             }
-            // Warps kWarps / 2 .. kWarps - 1 hand their sums to warps 0 .., and so on.  Named barriers of the two warps:
-            // 2 w - 1 says that warp w's buffer is full, 2 w that it is free again (w: among all compute warps).
-            bool mine = true;
-#pragma unroll
-            for (int from = Cfg::kWarps / 2; from > 0; from /= 2) {
-                if (part >= from && part < 2 * from) {
-                    float* to = join + ((group * (Cfg::kWarps - 1) + part - 1) * kHeads + g) * Cfg::kPadded + 2 * t;
-                    if (joined) {
-                        named_barrier_sync(2 * warp, 64);
-                    }
-                    if (t == 0) {
-                        bars.ml[warp][g] = make_float2(m, l);
-                    }
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        *reinterpret_cast<float2*>(to + i * 8) = make_float2(o[i][0], o[i][1]);
-                    }
-                    named_barrier_arrive(2 * warp - 1, 64);
-                    mine = false;
-                } else if (part < from) {
-                    const int other = warp + from;
-                    const float* at = join + ((group * (Cfg::kWarps - 1) + part + from - 1) * kHeads + g) * Cfg::kPadded + 2 * t;
-                    named_barrier_sync(2 * other - 1, 64);
-                    const float2 ml = bars.ml[other][g];
-                    const float most = fmaxf(m, ml.x), to = most == -INFINITY ? 0.0f : most;
-                    const float down = ex2(m - to), other_down = ex2(ml.x - to);
-                    l = l * down + ml.y * other_down;
-                    m = most;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const float2 x = *reinterpret_cast<const float2*>(at + i * 8);
-                        o[i][0] = o[i][0] * down + x.x * other_down;
-                        o[i][1] = o[i][1] * down + x.y * other_down;
-                    }
-                    named_barrier_arrive(2 * other, 64);
-                }
-            }
-            joined = true;
-            if (mine && head_here) {
-                if (walk.count == walk.units) {
-                    const int64_t row = (int64_t)walk.r * p.heads + kv * p.group + in_group;
-                    const float by = 1.0f / l;
-                    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + row * D) + t;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        out[i * 4] = pack<T>(o[i][0] * by, o[i][1] * by);
-                    }
-                    if (p.lse && t == 0) {
-                        p.lse[row] = ((m == -INFINITY ? 0.0f : m) - kShift + log2f(l)) * kLn2;
-                    }
-                } else {
-                    const int64_t row = ((int64_t)blockIdx.x * 2 + (walk.any ? 1 : 0)) * kUnitHeads + group * kHeads + g;
-                    float* out = p.part_o + row * D + 2 * t;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[i][0], o[i][1]);
-                    }
-                    if (t == 0) {
-                        p.part_ml[row] = make_float2(m, l);
-                    }
-                }
+            const int in_group = what.z + group * kHeads + g;
+            if ((which.w == 1 || join_parts(p, all, warp, next.x, which.w, flags & kFirstLater ? 1 : 0)) && in_group < p.group) {
+                write_result<T, D>(p, all, (int64_t)what.x * p.heads + what.y * p.group + in_group, part * kShare * 8);
             }
             __syncwarp();
         }
-        // the last buffers that were handed over have been taken (their barriers are left as they were found)
-        if (joined && part > 0) {
-            named_barrier_sync(2 * warp, 64);
-        }
         // requests without units: no keys, or lengths that cannot be
         for (int r = blockIdx.x; r < p.requests; r += gridDim.x) {
-            if (units_of<Cfg::kTile>(p, r) == 0) {
-                const bool empty = p.lengths[r] == 0;
-                const uint32_t fill = empty ? 0u : pack<T>(NAN, NAN);
+            const int len = length(r);
+            if (units_of<Cfg::kTile>(p, len) == 0) {
+                const uint32_t fill = len == 0 ? 0u : pack<T>(NAN, NAN);
                 uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + (int64_t)r * p.heads * D);
                 for (int i = threadIdx.x; i < p.heads * (D / 2); i += kComputeWarps * 32) {
                     o[i] = fill;
                 }
                 for (int i = threadIdx.x; p.lse && i < p.heads; i += kComputeWarps * 32) {
-                    p.lse[(int64_t)r * p.heads + i] = empty ? -INFINITY : NAN;
+                    p.lse[(int64_t)r * p.heads + i] = len == 0 ? -INFINITY : NAN;
                 }
             }
         }
-    }
-}
-
-// Joins the parts of one query head of a (request, head unit): block x of the first kernel named them in joins[x].  Most
-// blocks find nothing to join or a few parts, so a part is one warp's read and its maximum, sum and output are asked for
-// at once; of many parts each warp takes every fourth, and the warps are joined at the end.
-template <int D, typename T>
-__global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Params p, int unit_heads)
-{
-    constexpr int kWarps = kJoinThreads / 32, kPer = D / 32;
-    __shared__ float2 ml[kWarps];
-    __shared__ float sums[kWarps][D];
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const int4 j = p.joins[blockIdx.x];
-    const int h = blockIdx.y, head = (j.y % p.head_units) * unit_heads + h;
-    if (j.x < 0 || head >= p.group) {
-        return;
-    }
-    const int parts = j.z - (int)blockIdx.x + 2;  // of blocks blockIdx.x - 1 .. j.z
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    float m = -INFINITY, l = 0.0f, o[kPer] = {};
-    constexpr int kAtOnce = 4;
-    for (int i0 = warp; i0 < parts; i0 += kAtOnce * kWarps) {
-        float2 part[kAtOnce];
-        float x[kAtOnce][kPer];
-#pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            const int i = i0 + n * kWarps;
-            if (i < parts) {
-                const int64_t row = (((int64_t)blockIdx.x - 1 + i) * 2 + (i == 0 ? j.w : 0)) * unit_heads + h;
-                part[n] = p.part_ml[row];
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) {
-                    x[n][k] = p.part_o[row * D + lane + k * 32];
-                }
-            } else {
-                part[n] = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) {
-                    x[n][k] = 0.0f;
-                }
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            const float most = fmaxf(m, part[n].x), to = most == -INFINITY ? 0.0f : most;
-            const float down = ex2(m - to), other = ex2(part[n].x - to);
-            m = most;
-            l = l * down + part[n].y * other;
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                o[k] = o[k] * down + x[n][k] * other;
-            }
-        }
-    }
-    if (lane == 0) {
-        ml[warp] = make_float2(m, l);
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        sums[warp][lane + k * 32] = o[k];
-    }
-    __syncthreads();
-    float most = -INFINITY, total = 0.0f;
-    for (int w = 0; w < kWarps; ++w) {
-        most = fmaxf(most, ml[w].x);
-    }
-    const float to = most == -INFINITY ? 0.0f : most;
-    float weight[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        weight[w] = ex2(ml[w].x - to);
-        total += ml[w].y * weight[w];
-    }
-    const int64_t row = (int64_t)j.x * p.heads + (j.y / p.head_units) * p.group + head;
-    const float by = 1.0f / total;
-    if (threadIdx.x < D / 2) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            a += sums[w][2 * threadIdx.x] * weight[w];
-            b += sums[w][2 * threadIdx.x + 1] * weight[w];
-        }
-        reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + row * D)[threadIdx.x] = pack<T>(a * by, b * by);
-    }
-    if (p.lse && threadIdx.x == 0) {
-        p.lse[row] = (to - kShift + log2f(total)) * kLn2;
     }
 }
 
@@ -827,34 +963,18 @@ static int make_map(CUtensorMap* map, void* base, const spork_paged_cache& c, co
 }
 
 struct Workspace {
-    int64_t joins, ml, o, bytes;
+    int64_t ml, o, bytes;
     Workspace(int blocks, int groups, int D)
     {
-        const int64_t rows = (int64_t)blocks * 2 * groups * kHeads;
-        joins = 0;
-        ml = joins + (int64_t)blocks * 16;
+        const int64_t rows = (int64_t)blocks * 2 * kComputeWarps * kHeads;
+        ml = SPORK_ATTN_PAGED_COUNTERS;
         o = ml + rows * 8;
-        bytes = o + rows * D * 4;
+        bytes = o + rows * (D * groups / kComputeWarps) * 4;
     }
 };
 
-static cudaLaunchConfig_t launch_config(cudaLaunchAttribute* attr, dim3 grid, int threads, int smem, cudaStream_t stream)
-{
-    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr->val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cfg;
-}
-
 template <int D, typename T, typename Q, int kGroups>
-static int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, bool joined, DeviceState& dev,
-                  cudaStream_t stream)
+static int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, DeviceState& dev, cudaStream_t stream)
 {
     using Cfg = Config<D, kGroups>;
     auto kernel = attn_paged_kernel<D, T, Q, kGroups>;
@@ -866,33 +986,34 @@ static int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Para
     if (attr_err[dev.ordinal] != cudaSuccess) {
         return (int)attr_err[dev.ordinal];
     }
-    const int blocks = blocks_of(dev.sm_count);
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = launch_config(&attr, dim3(blocks), kThreads, Cfg::kSmem, stream);
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p);
-    if (e == cudaSuccess && joined) {
-        const int heads = p.group < kGroups * kHeads ? p.group : kGroups * kHeads;
-        cfg = launch_config(&attr, dim3(blocks, heads), kJoinThreads, 0, stream);
-        e = cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<D, T>, p, kGroups * kHeads);
-    }
-    return (int)e;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks_of(dev.sm_count));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p);
 }
 
 template <int D, typename T, typename Q>
-static int launch_groups(int groups, const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, bool joined,
+static int launch_groups(int groups, const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p,
                          DeviceState& dev, cudaStream_t stream)
 {
-    return groups == 1   ? launch<D, T, Q, 1>(map_k, map_v, p, joined, dev, stream)
-           : groups == 2 ? launch<D, T, Q, 2>(map_k, map_v, p, joined, dev, stream)
-                         : launch<D, T, Q, 4>(map_k, map_v, p, joined, dev, stream);
+    return groups == 1   ? launch<D, T, Q, 1>(map_k, map_v, p, dev, stream)
+           : groups == 2 ? launch<D, T, Q, 2>(map_k, map_v, p, dev, stream)
+                         : launch<D, T, Q, 4>(map_k, map_v, p, dev, stream);
 }
 
 template <int D, typename T>
-static int launch_q(bool f32, int groups, const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, bool joined,
+static int launch_q(bool f32, int groups, const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p,
                     DeviceState& dev, cudaStream_t stream)
 {
-    return f32 ? launch_groups<D, T, float>(groups, map_k, map_v, p, joined, dev, stream)
-               : launch_groups<D, T, T>(groups, map_k, map_v, p, joined, dev, stream);
+    return f32 ? launch_groups<D, T, float>(groups, map_k, map_v, p, dev, stream)
+               : launch_groups<D, T, T>(groups, map_k, map_v, p, dev, stream);
 }
 
 }  // namespace attn_paged_sm100
@@ -965,7 +1086,8 @@ extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* s
     }
     const int group = a.heads / c.kv_heads, groups = groups_of(group), blocks = blocks_of(dev->sm_count);
     const Workspace w(blocks, groups, c.head_dim);
-    if (blocks > kMaxBlocks) {
+    static_assert(kFan * kFan * kFan * kFan >= kMaxBlocks && kLevels == 4, "levels of joining");
+    if (blocks > kMaxBlocks || (int64_t)kLevels * blocks * 2 * kComputeWarps * 4 > SPORK_ATTN_PAGED_COUNTERS) {
         return SPORK_ERR_TOO_LARGE;
     }
     if (!a.workspace || a.workspace_bytes < w.bytes) {
@@ -991,25 +1113,28 @@ extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* s
     p.kv_heads = c.kv_heads;
     p.group = group;
     p.head_units = (group + groups * kHeads - 1) / (groups * kHeads);
-    p.max_blocks = a.max_blocks;
+    const int64_t capacity = (int64_t)a.max_blocks * c.page_size;
+    p.capacity = capacity < 0x7FFFFFFF ? (int32_t)capacity : 0x7FFFFFFF;
+    // places in the list of units, at most
+    if (((p.capacity >> 6) + 1 + kPairCost) * (int64_t)a.requests * c.kv_heads * p.head_units > 0x7FFFFFFF) {
+        return SPORK_ERR_TOO_LARGE;
+    }
     p.num_pages = c.num_pages;
     p.page_size = c.page_size;
     p.box_rows = c.page_size < kMaxRows ? c.page_size : kMaxRows;
     p.scale_log2e = a.scale * kLog2e;
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-    p.joins = reinterpret_cast<int4*>(ws + w.joins);
+    p.arrived = reinterpret_cast<uint32_t*>(ws);
     p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
     p.part_o = reinterpret_cast<float*>(ws + w.o);
     p.status = dev->status_word;
     p.q_pairs = ((reinterpret_cast<uintptr_t>(a.q) % (2 * q_elem)) | ((a.q_request_stride | a.q_head_stride) & 1)) == 0;
-    // one unit at most for every request: nothing to join
-    const bool joined = (int64_t)a.max_blocks * c.page_size > 8192 / c.head_dim;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f32 = a.q_type == SPORK_TYPE_F32;
     if (c.type == SPORK_TYPE_F16) {
-        return c.head_dim == 64 ? launch_q<64, __half>(f32, groups, map_k, map_v, p, joined, *dev, s)
-                                : launch_q<128, __half>(f32, groups, map_k, map_v, p, joined, *dev, s);
+        return c.head_dim == 64 ? launch_q<64, __half>(f32, groups, map_k, map_v, p, *dev, s)
+                                : launch_q<128, __half>(f32, groups, map_k, map_v, p, *dev, s);
     }
-    return c.head_dim == 64 ? launch_q<64, __nv_bfloat16>(f32, groups, map_k, map_v, p, joined, *dev, s)
-                            : launch_q<128, __nv_bfloat16>(f32, groups, map_k, map_v, p, joined, *dev, s);
+    return c.head_dim == 64 ? launch_q<64, __nv_bfloat16>(f32, groups, map_k, map_v, p, *dev, s)
+                            : launch_q<128, __nv_bfloat16>(f32, groups, map_k, map_v, p, *dev, s);
 }

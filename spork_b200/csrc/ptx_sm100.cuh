@@ -781,12 +781,6 @@ __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t threads
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Counts this warp in at the barrier without waiting at it.
-__device__ __forceinline__ void named_barrier_arrive(uint32_t id, uint32_t threads)
-{
-    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 // ----------------------------------------------------------- checked build ---
 
 // Range checks of a debug build (-DSPORK_CHECKED): every shared-memory address handed to TMA, to an MMA

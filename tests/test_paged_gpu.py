@@ -359,14 +359,16 @@ def test_attention_writes_its_outputs_and_nothing_else(sp, cuda):
     before = [t.clone() for t in (case.q, case.kc, case.vc, case.table, case.len)]
     need = sp.attn_paged_workspace(8, 4, 64)
     work = torch.full((need + 64,), 123, dtype=torch.uint8, device=cuda)
-    o, lse = case.run(sp, o=room[64:-64].view(4, 8, 64), workspace=work[:need])
-    case.check(o, lse)
+    work[:65536] = 0
+    for _ in range(3):
+        o, lse = case.run(sp, o=room[64:-64].view(4, 8, 64), workspace=work[:need])
+        case.check(o, lse)
+        assert (work[:65536] == 0).all()
     assert (room[:64] == 9).all() and (room[-64:] == 9).all() and (work[need:] == 123).all()
     for t, b in zip((case.q, case.kc, case.vc, case.table, case.len), before):
         assert torch.equal(t.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
-    if need:
-        with pytest.raises(sp.SporkError):
-            case.run(sp, workspace=work[:need - 16])
+    with pytest.raises(sp.SporkError):
+        case.run(sp, workspace=work[:need - 16])
 
 
 def test_attention_is_the_same_in_every_run(sp, cuda):
