@@ -471,18 +471,19 @@ _PAGED_ATTN_ARGS = struct.Struct("=" + _CACHE + "6Q4q4ifi")
 # kernels of a few microseconds, so they look each property of a tensor up once and call as little as they can
 _T = None
 _TYPE_CODES: dict = {}
-_current_device = _raw_stream = None
+_current_device = _raw_stream = _capturing = None
 _workspace_bytes: dict = {}  # by device and what the size depends on
 _workspaces: dict = {}       # by device and stream: the one that calls without a workspace of their own use
 _COUNTER_BYTES = 65536       # SPORK_ATTN_PAGED_COUNTERS
 
 
 def _bind_torch():
-    global _T, _current_device, _raw_stream
+    global _T, _current_device, _raw_stream, _capturing
     import torch
 
     _TYPE_CODES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
     _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _capturing = torch._C._cuda_isCurrentStreamCapturing
     _T = torch
     return torch
 
@@ -499,19 +500,21 @@ def _on_gpu(**tensors) -> None:
             raise ValueError(f"tensors are on different devices: {first} on {device}, {name} on {t.get_device()}")
 
 
-def _launch(fn, packed: bytes, device: int, stream, what: str) -> None:
-    """Launch on the given stream, which must be of the tensors' device, or on that device's current one."""
+def _stream_of(stream, device: int) -> int:
+    """The given stream, which must be of the tensors' device, or that device's current one."""
     if stream is None:
-        sp = _raw_stream(device)
-    elif stream.device_index != device:
+        return _raw_stream(device)
+    if stream.device_index != device:
         raise ValueError(f"the stream is of device {stream.device_index}, the tensors of device {device}")
-    else:
-        sp = stream.cuda_stream
+    return stream.cuda_stream
+
+
+def _call(fn, packed: bytes, device: int, stream: int, what: str) -> None:
     if _current_device() == device:
-        rc = fn(packed, sp)
+        rc = fn(packed, stream)
     else:
         with _T.cuda.device(device):
-            rc = fn(packed, sp)
+            rc = fn(packed, stream)
     if rc:
         raise SporkError(rc, what)
 
@@ -524,32 +527,28 @@ def _new(like, shape, dtype, stream):
         return _T.empty(shape, dtype=dtype, device=like.device)
 
 
-def _workspace(like, device: int, need: int, stream):
-    """A workspace for one launch.  Launches of one stream follow one another and share the stream's; a captured launch, whose
-    graph may be replayed beside any other, gets one of its own, with the clearing of its counters in the graph."""
-    key = (device, _raw_stream(device) if stream is None else stream.cuda_stream)
-    if _T.cuda.is_current_stream_capturing() if stream is None else _capturing(stream):
-        workspace = _new(like, (need,), _T.uint8, stream)
-        if stream is None:
-            workspace[:_COUNTER_BYTES].zero_()
-        else:
-            with _T.cuda.stream(stream):
-                workspace[:_COUNTER_BYTES].zero_()
+def _own_workspace(like, device: int, stream, key):
+    """The workspace of one launch that was not given any.  Launches of one stream follow one another and share the stream's;
+    a captured launch, whose graph may be replayed beside any other, gets one of its own, with the clearing of its counters
+    in the graph."""
+    if stream is not None:
+        with _T.cuda.stream(stream):
+            return _own_workspace(like, device, None, key)
+    if _current_device() != device:
+        with _T.cuda.device(device):
+            return _own_workspace(like, device, None, key)
+    need = _workspace_bytes.get(key)
+    if need is None:
+        need = _workspace_bytes[key] = attn_paged_workspace(*key[1:])
+    if _capturing():
+        workspace = _T.empty((need,), dtype=_T.uint8, device=like.device)
+        workspace[:_COUNTER_BYTES].zero_()
         return workspace
-    workspace = _workspaces.get(key)
+    at = (device, _raw_stream(device))
+    workspace = _workspaces.get(at)
     if workspace is None or workspace.numel() < need:
-        if stream is None:
-            workspace = _T.zeros((need,), dtype=_T.uint8, device=like.device)
-        else:
-            with _T.cuda.stream(stream):
-                workspace = _T.zeros((need,), dtype=_T.uint8, device=like.device)
-        _workspaces[key] = workspace
+        workspace = _workspaces[at] = _T.zeros((need,), dtype=_T.uint8, device=like.device)
     return workspace
-
-
-def _capturing(stream) -> bool:
-    with _T.cuda.stream(stream):
-        return _T.cuda.is_current_stream_capturing()
 
 
 def _vector(t, n, dtype, what: str):
@@ -612,10 +611,14 @@ def paged_tables(lengths, new_tokens, block_table, free_pages, free_used, *, pag
     if len(shape) != 1:
         raise ValueError(f"lengths must be (R,), got {tuple(shape)}")
     n = shape[0]
-    _vector(lengths, n, i32, "lengths")
-    _vector(new_tokens, n, i32, "new_tokens")
-    _vector(free_pages, None, i32, "free_pages")
-    _vector(free_used, 1, i32, "free_used")
+    # (looked at together, and one by one only to say what is wrong)
+    if not (lengths.dtype is i32 and new_tokens.dtype is i32 and free_pages.dtype is i32 and free_used.dtype is i32
+            and new_tokens.shape == shape and lengths.is_contiguous() and new_tokens.is_contiguous()
+            and free_pages.is_contiguous() and free_used.shape == (1,) and len(free_pages.shape) == 1):
+        _vector(lengths, n, i32, "lengths")
+        _vector(new_tokens, n, i32, "new_tokens")
+        _vector(free_pages, None, i32, "free_pages")
+        _vector(free_used, 1, i32, "free_used")
     blocks, row = _block_table(block_table, n)
     if not 1 <= page_size < 1 << 31:
         raise ValueError(f"page_size must be at least 1 and below 2^31, got {page_size}")
@@ -638,7 +641,7 @@ def paged_tables(lengths, new_tokens, block_table, free_pages, free_used, *, pag
         lengths.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_used.data_ptr(),
         slots.data_ptr(), offsets.data_ptr(), lengths_after.data_ptr(), info.data_ptr(), row, slots.shape[0], n, blocks,
         page_size, free_pages.shape[0])
-    _launch((_lib or lib()).spork_paged_sm100_tables, packed, device, stream, "spork_paged_sm100_tables")
+    _call((_lib or lib()).spork_paged_sm100_tables, packed, device, _stream_of(stream, device), "spork_paged_sm100_tables")
     return slots, offsets, lengths_after, info
 
 
@@ -662,14 +665,15 @@ def paged_store(k, v, k_cache, v_cache, slots, stream=None):
     kn, vn = k.stride(), v.stride()
     if (kn[2] != 1 or vn[2] != 1) and dim > 1:
         raise ValueError("the head dimension of k and v must be contiguous")
-    _vector(slots, tokens[0], torch.int64, "slots")
+    if slots.dtype is not torch.int64 or slots.shape != tokens[:1] or not slots.is_contiguous():
+        _vector(slots, tokens[0], torch.int64, "slots")
     device = k_cache.get_device()
     if device < 0 or not (device == v_cache.get_device() == k.get_device() == v.get_device() == slots.get_device()):
         _on_gpu(k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots)
     packed = _STORE_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], code, pages, kv_heads, page, dim, 0,
         k.data_ptr(), v.data_ptr(), slots.data_ptr(), kn[0], kn[1], vn[0], vn[1], tokens[0], src, 0)
-    _launch((_lib or lib()).spork_paged_sm100_store, packed, device, stream, "spork_paged_sm100_store")
+    _call((_lib or lib()).spork_paged_sm100_store, packed, device, _stream_of(stream, device), "spork_paged_sm100_store")
 
 
 def attn_paged_supports(heads: int, kv_heads: int, head_dim: int, page_size: int) -> bool:
@@ -714,7 +718,8 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     if qs[2] != 1:
         raise ValueError("the head dimension of q must be contiguous")
     blocks, row = _block_table(block_table, n)
-    _vector(lengths, n, torch.int32, "lengths")
+    if lengths.dtype is not torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous():
+        _vector(lengths, n, torch.int32, "lengths")
     if o is None:
         o = _new(q, (n, heads, dim), dtype, stream)
     elif o.shape != q_shape:
@@ -733,16 +738,10 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
                           == lengths.get_device() == o.get_device()) or (lse is not None and lse.get_device() != device):
         _on_gpu(q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, o=o,
                 **({} if lse is None else {"lse": lse}))
+    launch_stream = _stream_of(stream, device)
     if workspace is None:
-        key = (device, heads, kv_heads, dim)
-        need = _workspace_bytes.get(key)
-        if need is None:
-            with _OnDevice(device):
-                need = _workspace_bytes[key] = attn_paged_workspace(heads, kv_heads, dim)
-        workspace = _workspace(q, device, need, stream)
-        need = workspace.numel()
+        workspace = _own_workspace(q, device, stream, (device, heads, kv_heads, dim))
     else:
-        need = workspace.numel() * workspace.element_size()
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
         if workspace.get_device() != device:
@@ -750,7 +749,7 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     packed = _PAGED_ATTN_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], code, pages, kv_heads, page, dim, 0,
         q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        workspace.data_ptr(), need, qs[0], qs[1], row, n, heads, blocks, q_code,
+        workspace.data_ptr(), workspace.nbytes, qs[0], qs[1], row, n, heads, blocks, q_code,
         1.0 / dim ** 0.5 if scale is None else scale, 0)
-    _launch((_lib or lib()).spork_attn_sm100_paged, packed, device, stream, "spork_attn_sm100_paged")
+    _call((_lib or lib()).spork_attn_sm100_paged, packed, device, launch_stream, "spork_attn_sm100_paged")
     return o
