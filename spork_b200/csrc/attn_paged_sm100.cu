@@ -113,11 +113,11 @@ constexpr int kDone = 1, kLater = 2, kFirstLater = 4, kBad = 8;
 
 struct Bars {
     uint64_t full[4], empty[4];
-    uint64_t handed[kComputeWarps], taken[kComputeWarps];  // what others have for a warp is there; the warp has taken it
+    uint64_t handed[kComputeWarps], taken[kComputeWarps];  // a group's warps have handed over, and taken, what is for each
     Note note[4];
     uint32_t warp_sums[8];
     uint32_t start[3];       // the block's first (request, head unit): request, which head unit, its place in the list
-    float2 ml[kComputeWarps][kComputeWarps][kHeads];  // [to][from]: maxima and sums
+    float2 ml[kComputeWarps][kHeads];  // each warp's maxima and sums
     int32_t lengths[kLengths];  // of the first requests
     uint32_t abort_flag;
 };
@@ -243,17 +243,6 @@ __device__ __forceinline__ void report_timeout(const Params& p, volatile uint32_
     atomicCAS(p.status, 0u, 0x90000000u | (role << 24) | ((where & 0xFFu) << 16) | (blockIdx.x & 0xFFFFu));
 }
 
-// Two neighbouring elements of q; `pairs`: they may be read at once.
-__device__ __forceinline__ float2 load_two(const float* q, bool pairs)
-{
-    return pairs ? *reinterpret_cast<const float2*>(q) : make_float2(q[0], q[1]);
-}
-__device__ __forceinline__ uint32_t load_two(const void* q, bool pairs)
-{
-    const uint16_t* x = static_cast<const uint16_t*>(q);
-    return pairs ? *reinterpret_cast<const uint32_t*>(q) : x[0] | (uint32_t)x[1] << 16;
-}
-
 // What one warp has of its 8 query heads and a run of keys: maxima, sums, unnormalised output (fragments: row g of the
 // first product's operand is in [0], [1], row g + 8, its low part, in [2], [3]); and the weights of the unit at hand.
 template <int D, typename T, bool kLowQ, int kKeys>
@@ -265,20 +254,31 @@ struct Softmax {
     float m, l;  // of row g; l: this lane's columns only
     uint32_t weights[kPairs][4];
 
-    // The queries as they are (kLowQ: 32 bits), on their way into the registers that begin() makes operands of.
+    // The queries as they are (kLowQ: 32 bits), on their way into the registers that begin() makes operands of.  Nothing is
+    // done with what is loaded, so that nothing waits for it here.  `pairs`: two neighbours may be read at once.
     template <typename Q>
-    __device__ __forceinline__ void ask_for(const Q* q, bool here, bool pairs)
+    __device__ __forceinline__ void ask_for(const Q* q, bool pairs)
     {
+        if (pairs) {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int i = 0; i < 2 * kSteps; ++i) {
                 if constexpr (kLowQ) {
-                    const float2 x = here ? load_two(q + i * 16 + j * 8, pairs) : make_float2(0.0f, 0.0f);
-                    q_hi[i][j] = __float_as_uint(x.x);
-                    q_lo[i][j] = __float_as_uint(x.y);
+                    const uint2 x = *reinterpret_cast<const uint2*>(q + i * 8);
+                    q_hi[i / 2][i % 2] = x.x;
+                    q_lo[i / 2][i % 2] = x.y;
                 } else {
-                    q_hi[i][j] = here ? load_two(q + i * 16 + j * 8, pairs) : 0u;
+                    q_hi[i / 2][i % 2] = *reinterpret_cast<const uint32_t*>(q + i * 8);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i) {
+                if constexpr (kLowQ) {
+                    q_hi[i / 2][i % 2] = reinterpret_cast<const uint32_t*>(q)[i * 8];
+                    q_lo[i / 2][i % 2] = reinterpret_cast<const uint32_t*>(q)[i * 8 + 1];
+                } else {
+                    const uint16_t* x = reinterpret_cast<const uint16_t*>(q) + i * 8;
+                    q_hi[i / 2][i % 2] = x[0] | (uint32_t)x[1] << 16;
                 }
             }
         }
@@ -350,14 +350,17 @@ struct Softmax {
             most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
             most = fmaxf(most, m);
             const float down = ex2(m - (most == -INFINITY ? 0.0f : most));
+            const bool nothing_yet = __all_sync(0xFFFFFFFFu, m == -INFINITY);
             m = most;
-            l *= down;
+            if (!nothing_yet) {
+                l *= down;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                acc[i][0] *= down;
-                acc[i][1] *= down;
-                acc[i][2] *= down;
-                acc[i][3] *= down;
+                for (int i = 0; i < D / 8; ++i) {
+                    acc[i][0] *= down;
+                    acc[i][1] *= down;
+                    acc[i][2] *= down;
+                    acc[i][3] *= down;
+                }
             }
         }
         const float shift = m == -INFINITY ? 0.0f : kShift - m;
@@ -546,9 +549,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             mbar_init(smem_u32(&bars.full[s]), 1);
             mbar_init(smem_u32(&bars.empty[s]), kComputeWarps);
         }
-        for (int w = 0; w < kComputeWarps; ++w) {
-            mbar_init(smem_u32(&bars.handed[w]), Cfg::kWarps > 1 ? Cfg::kWarps - 1 : 1);
-            mbar_init(smem_u32(&bars.taken[w]), 1);
+        for (int g = 0; g < kGroups; ++g) {
+            mbar_init(smem_u32(&bars.handed[g]), Cfg::kWarps);
+            mbar_init(smem_u32(&bars.taken[g]), Cfg::kWarps);
         }
         bars.abort_flag = 0;
         fence_mbar_init();
@@ -752,11 +755,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         constexpr int kPairs = S::kPairs, kChunks = Cfg::kKeys / Cfg::kChunk;
         S sm;
         auto ask_for = [&](int r, int kv, int head) {
+            // (rows of heads that do not exist get the first one's queries; nobody looks at what they come to)
             const int in_group = head + group * kHeads + g;
-            const bool here = in_group < p.group;
             sm.ask_for(static_cast<const Q*>(p.q) + r * p.q_request_stride +
-                           (int64_t)(kv * p.group + (here ? in_group : 0)) * p.q_head_stride + 2 * t,
-                       here, p.q_pairs);
+                           (int64_t)(kv * p.group + (in_group < p.group ? in_group : 0)) * p.q_head_stride + 2 * t,
+                       p.q_pairs);
         };
         if (more) {
             ask_for(walk.r, walk.kv, walk.hu * kUnitHeads);
@@ -842,57 +845,55 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             Part<kShare> all;
             all.m = sm.m;
             all.l = l;
+            if (kWarps > 1) {
+                ok = wait(&bars.taken[group], (times & 1u) ^ 1u, 3, group);
+                if (!ok) {
+                    break;
+                }
+            }
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const int to = group * kWarps + w;
-                if (w == part) {
+                float* row = handed + (to * (kWarps - 1) + (part < w ? part : part - 1)) * Cfg::kHanded + g * kShare * 8 + 2 * t;
 #pragma unroll
-                    for (int i = 0; i < kShare; ++i) {
-                        const float(&a)[4] = sm.acc[w * kShare + i];
-                        all.o[i] = make_float2(a[0] + a[2], a[1] + a[3]);
-                    }
-                } else {
-                    ok = ok && wait(&bars.taken[to], (times & 1u) ^ 1u, 3, to);
-                    if (ok) {
-                        float* row = handed + (to * (kWarps - 1) + (part < w ? part : part - 1)) * Cfg::kHanded + g * kShare * 8 + 2 * t;
-#pragma unroll
-                        for (int i = 0; i < kShare; ++i) {
-                            const float(&a)[4] = sm.acc[w * kShare + i];
-                            *reinterpret_cast<float2*>(row + turned(i) * 8) = make_float2(a[0] + a[2], a[1] + a[3]);
-                        }
-                        if (t == 0) {
-                            bars.ml[to][warp][g] = make_float2(sm.m, l);
-                        }
-                        __syncwarp();
-                        if (lane == 0) {
-                            mbar_arrive(smem_u32(&bars.handed[to]));
-                        }
+                for (int i = 0; i < kShare; ++i) {
+                    const float(&a)[4] = sm.acc[w * kShare + i];
+                    const float2 o = make_float2(a[0] + a[2], a[1] + a[3]);
+                    if (w == part) {
+                        all.o[i] = o;
+                    } else {
+                        *reinterpret_cast<float2*>(row + turned(i) * 8) = o;
                     }
                 }
             }
             if (kWarps > 1) {
-                ok = ok && wait(&bars.handed[warp], times & 1u, 4, warp);
-                if (ok) {
+                if (t == 0) {
+                    bars.ml[warp][g] = make_float2(sm.m, l);
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&bars.handed[group]));
+                }
+                ok = wait(&bars.handed[group], times & 1u, 4, group);
+                if (!ok) {
+                    break;
+                }
 #pragma unroll
-                    for (int w = 0; w < kWarps - 1; ++w) {
-                        const float* row = handed + (warp * (kWarps - 1) + w) * Cfg::kHanded + g * kShare * 8 + 2 * t;
-                        const float2 ml = bars.ml[warp][group * kWarps + (w < part ? w : w + 1)][g];
-                        float2 o[kShare];
+                for (int w = 0; w < kWarps - 1; ++w) {
+                    const float* row = handed + (warp * (kWarps - 1) + w) * Cfg::kHanded + g * kShare * 8 + 2 * t;
+                    const float2 ml = bars.ml[group * kWarps + (w < part ? w : w + 1)][g];
+                    float2 o[kShare];
 #pragma unroll
-                        for (int i = 0; i < kShare; ++i) {
-                            o[i] = *reinterpret_cast<const float2*>(row + turned(i) * 8);
-                        }
-                        all.join(ml.x, ml.y, o);
+                    for (int i = 0; i < kShare; ++i) {
+                        o[i] = *reinterpret_cast<const float2*>(row + turned(i) * 8);
                     }
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&bars.taken[warp]));
-                    }
+                    all.join(ml.x, ml.y, o);
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&bars.taken[group]));
                 }
                 ++times;
-            }
-            if (!ok) {
-                break;
             }
             const int in_group = what.z + group * kHeads + g;
             if ((which.w == 1 || join_parts(p, all, warp, next.x, which.w, flags & kFirstLater ? 1 : 0)) && in_group < p.group) {
