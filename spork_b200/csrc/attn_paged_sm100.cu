@@ -48,7 +48,7 @@ constexpr int kHeads = 8;          // query heads of a group of warps
 // weights are 2^(x - max + 6), and max may be out of date by 8: up to 2^14, within fp16, whose small weights stay normal
 constexpr float kShift = 6.0f, kSlack = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMaxBlocks = 1024;   // blocks of a launch
+constexpr int kMaxBlocks = 512;    // blocks of a launch
 constexpr int kComputeWarps = 4;
 // the computing warps, the copying one, and three idle ones that complete the second warpgroup, so that whole warpgroups
 // can trade registers
@@ -62,8 +62,8 @@ constexpr int kWhole = 4;          // a (request, key head) of so many units or 
 constexpr int kMinRun = 2;         // places of a block's run, at least
 constexpr int kMaxRows = 64;       // rows of a TMA box
 constexpr int kLengths = 512;      // requests whose lengths a block keeps in shared memory
-constexpr int kFan = 8;            // parts that are joined at a time
-constexpr int kLevels = 4;         // of joining: kFan^kLevels is more than the blocks of a launch
+constexpr int kFan = 10;           // parts that are joined at a time
+constexpr int kLevels = 3;         // of joining: kFan^kLevels is more than the blocks of a launch
 
 // kGroups groups of warps share a unit, each with 8 query heads of its own.
 template <int D, int kGroups>
@@ -74,7 +74,9 @@ struct Config {
     static constexpr int kChunk = kKeys < 32 ? kKeys : 32;      // taken at once
     static constexpr int kHalfUnit = kTile * D * 2;             // the keys (or values) of a unit, bytes
     static constexpr int kStageBytes = 2 * kHalfUnit;
-    static constexpr int kStages = 3;
+    // Two: with three the loads of SMs that are served better crowd out those of the others, and equal runs end up to a
+    // fifth of their time apart (16 requests of 4096 keys, 16 heads of 128: 89.0 us with three, 85.6 with two).
+    static constexpr int kStages = 2;
     static constexpr int kShare = D / 8 / kWarps;               // groups of 8 columns that a warp joins
     static constexpr int kHanded = kHeads * kShare * 8;         // floats from one warp to another
     static constexpr int kSmem = 1024 + kStages * kStageBytes + kComputeWarps * (kWarps - 1) * kHanded * 4;
@@ -295,6 +297,10 @@ struct Softmax {
                 }
             }
         }
+    }
+
+    __device__ __forceinline__ void clear()
+    {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
             acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
@@ -438,96 +444,105 @@ struct Part {
     }
 };
 
-// Row `row` of the output: the share's columns from `column` on.
-template <typename T, int D, int kShare>
-__device__ __forceinline__ void write_result(const Params& p, const Part<kShare>& all, int64_t row, int column)
+// A row of the output: the share's columns from `o` on, and where `lse` is not null the logarithm of the sum.
+template <typename T, int kShare>
+__device__ __forceinline__ void write_result(const Part<kShare>& all, T* o, float* lse)
 {
     const int t = threadIdx.x % 4;
     const float by = 1.0f / all.l;
-    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + row * D + column) + t;
+    uint32_t* out = reinterpret_cast<uint32_t*>(o) + t;
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
         out[i * 4] = pack<T>(all.o[i].x * by, all.o[i].y * by);
     }
-    if (p.lse && t == 0 && column == 0) {
-        p.lse[row] = ((all.m == -INFINITY ? 0.0f : all.m) - kShift + log2f(all.l)) * kLn2;
+    if (lse && t == 0) {
+        *lse = ((all.m == -INFINITY ? 0.0f : all.m) - kShift + log2f(all.l)) * kLn2;
     }
 }
 
+// A part in the workspace: [warp][head], maxima and sums, and [warp][head][the warp's share of D].
 template <int kShare>
-__device__ __forceinline__ void write_part(const Params& p, const Part<kShare>& all, int64_t row)
+__device__ __forceinline__ void write_part(const Part<kShare>& all, float2* part_ml, float* part_o, uint32_t row)
 {
     const int t = threadIdx.x % 4;
-    float* out = p.part_o + row * (kShare * 8) + 2 * t;
+    float* out = part_o + row * (kShare * 8) + 2 * t;
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
         __stcg(reinterpret_cast<float2*>(out + i * 8), all.o[i]);
     }
     if (t == 0) {
-        __stcg(p.part_ml + row, make_float2(all.m, all.l));
+        __stcg(part_ml + row, make_float2(all.m, all.l));
     }
 }
 
-// A warp writes its share of this block's part, and counts it in.  The parts are those of blocks first .. first + parts - 1
-// (the first one in that block's slot first_slot, the others in slot 0).  The last of every kFan joins these in order and
-// leaves the result where the first of them was, and so on; the last of all returns true with the whole.
-template <int kShare>
-__device__ __forceinline__ bool join_parts(const Params& p, Part<kShare>& all, int warp, int first, int parts, int first_slot)
+// Where part i of those of blocks first .. is: the first one in that block's slot first_slot, the others in slot 0.
+__device__ __forceinline__ uint32_t place_of(int first, int first_slot, int i)
+{
+    return ((first + i) * 2 + (i == 0 ? first_slot : 0)) * kComputeWarps + threadIdx.x / 32;
+}
+
+// A warp counts its share of this block's part in, which it has written.  The last of every kFan joins these in order and
+// leaves the result where the first of them was, and so on; the last of all writes the row of the output (o null: there is
+// none). 
+// (Few parts are under way at a time: the main loop's registers are all in use, and it bears no spills.  With 200 bytes of
+// them to a thread the kernel took up to 1.4 times as long: beside the stages little of L1 is left to keep them.)
+template <typename T, int kShare>
+__device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, float* part_o, int first, int parts, int first_slot,
+                                        T* o, float* lse)
 {
     const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    auto place = [&](int i) { return ((int64_t)(first + i) * 2 + (i == 0 ? first_slot : 0)) * kComputeWarps + warp; };
-    auto row_of = [&](int i) { return place(i) * kHeads + g; };
     int mine = (int)blockIdx.x - first, step = 1;  // part i of a level is where part i * step of the lowest one was
-    bool written = false;
-    for (int n = parts, level = 0; n > 1; n = (n + kFan - 1) / kFan, ++level, step *= kFan, mine /= kFan) {
-        if (!written) {
-            write_part(p, all, row_of(mine * step));
-            written = true;
-        }
+    for (int n = parts; n > 1; n = (n + kFan - 1) / kFan, step *= kFan, mine /= kFan) {
         const int begin = mine / kFan * kFan, members = n - begin < kFan ? n - begin : kFan;
-        if (members == 1) {
-            continue;  // it is its own join, where it is
-        }
-        uint32_t* counter = p.arrived + (int64_t)level * gridDim.x * 2 * kComputeWarps + place(begin * step);
-        __syncwarp();
-        uint32_t before = 0;
-        if (lane == 0) {
-            // releases what the warp has written, and acquires what the others had when they counted themselves in
-            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
-        }
-        before = __shfl_sync(0xFFFFFFFFu, before, 0);
-        __syncwarp();
-        if (before != (uint32_t)members - 1u) {
-            return false;
-        }
-        if (lane == 0) {
-            *counter = 0u;  // for the next launch
-        }
-        all.clear();
-        constexpr int kAtOnce = kShare <= 4 ? 4 : kShare == 8 ? 2 : 1;
-        for (int k = 0; k < members; k += kAtOnce) {
-            float2 ml[kAtOnce], o[kAtOnce][kShare];
+        if (members > 1) {
+            uint32_t* counter = arrived + place_of(first, first_slot, begin * step);
+            __syncwarp();
+            uint32_t before = 0;
+            if (lane == 0) {
+                // releases what the warp has written, and acquires what the others had when they counted themselves in
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+            }
+            before = __shfl_sync(0xFFFFFFFFu, before, 0);
+            __syncwarp();
+            if (before != (uint32_t)members - 1u) {
+                return;
+            }
+            if (lane == 0) {
+                *counter = 0u;  // for the next launch
+            }
+            Part<kShare> all;
+            all.clear();
+            constexpr int kAtOnce = kShare <= 4 ? 2 : 1;
+            for (int k = 0; k < members; k += kAtOnce) {
+                float2 ml[kAtOnce], x[kAtOnce][kShare];
 #pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {
-                if (x == 0 || k + x < members) {
-                    const int64_t from = row_of((begin + k + x) * step);
-                    ml[x] = __ldcg(p.part_ml + from);
+                for (int j = 0; j < kAtOnce; ++j) {
+                    if (j == 0 || k + j < members) {
+                        const uint32_t row = place_of(first, first_slot, (begin + k + j) * step) * kHeads + g;
+                        ml[j] = __ldcg(part_ml + row);
 #pragma unroll
-                    for (int i = 0; i < kShare; ++i) {
-                        o[x][i] = __ldcg(reinterpret_cast<const float2*>(p.part_o + from * (kShare * 8) + 2 * t + i * 8));
+                        for (int i = 0; i < kShare; ++i) {
+                            x[j][i] = __ldcg(reinterpret_cast<const float2*>(part_o + row * (kShare * 8) + 2 * t + i * 8));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    if (j == 0 || k + j < members) {
+                        all.join(ml[j].x, ml[j].y, x[j]);
                     }
                 }
             }
-#pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {
-                if (x == 0 || k + x < members) {
-                    all.join(ml[x].x, ml[x].y, o[x]);
+            if (n <= kFan) {
+                if (o) {
+                    write_result(all, o, lse);
                 }
+                return;
             }
+            write_part(all, part_ml, part_o, place_of(first, first_slot, begin * step) * kHeads + g);
         }
-        written = false;
+        arrived += gridDim.x * 2 * kComputeWarps;  // (one alone is its own join, where it is)
     }
-    return true;
 }
 
 template <int D, typename T, typename Q, int kGroups>
@@ -541,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     __shared__ Bars bars;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t stages = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    float* handed = reinterpret_cast<float*>(smem_raw + (stages - smem_u32(smem_raw)) + Cfg::kStages * Cfg::kStageBytes);
+    const uint32_t handed = stages + Cfg::kStages * Cfg::kStageBytes;
     volatile uint32_t* abort_flag = &bars.abort_flag;
 
     if (threadIdx.x == 0) {
@@ -754,6 +769,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         using S = Softmax<D, T, kLowQ, Cfg::kChunk>;
         constexpr int kPairs = S::kPairs, kChunks = Cfg::kKeys / Cfg::kChunk;
         S sm;
+        sm.clear();
         auto ask_for = [&](int r, int kv, int head) {
             // (rows of heads that do not exist get the first one's queries; nobody looks at what they come to)
             const int in_group = head + group * kHeads + g;
@@ -840,8 +856,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
             l = bad ? NAN : l;
             constexpr int kWarps = Cfg::kWarps, kShare = Cfg::kShare;
-            // groups of 8 columns change places by row, so that no two rows' meet in a bank
-            auto turned = [&](int i) { return i ^ ((kShare == 2 ? g >> 1 : g) & (kShare - 1)); };
+            // where row g of what warp `from` has for warp `to` is; groups of 8 columns change places by row (their number
+            // is xored to it), so that no two rows' meet in a bank
+            auto handed_at = [&](int to, int from) {
+                return handed + ((group * kWarps + to) * (kWarps - 1) + (from < to ? from : from - 1)) * (Cfg::kHanded * 4) +
+                       (g * kShare + ((kShare == 2 ? g >> 1 : g) & (kShare - 1))) * 32 + t * 8;
+            };
             Part<kShare> all;
             all.m = sm.m;
             all.l = l;
@@ -853,8 +873,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             }
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const int to = group * kWarps + w;
-                float* row = handed + (to * (kWarps - 1) + (part < w ? part : part - 1)) * Cfg::kHanded + g * kShare * 8 + 2 * t;
+                const uint32_t row = handed_at(w, part);
 #pragma unroll
                 for (int i = 0; i < kShare; ++i) {
                     const float(&a)[4] = sm.acc[w * kShare + i];
@@ -862,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                     if (w == part) {
                         all.o[i] = o;
                     } else {
-                        *reinterpret_cast<float2*>(row + turned(i) * 8) = o;
+                        st_shared_f2(row ^ (i * 32), o);
                     }
                 }
             }
@@ -880,12 +899,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                 }
 #pragma unroll
                 for (int w = 0; w < kWarps - 1; ++w) {
-                    const float* row = handed + (warp * (kWarps - 1) + w) * Cfg::kHanded + g * kShare * 8 + 2 * t;
-                    const float2 ml = bars.ml[group * kWarps + (w < part ? w : w + 1)][g];
+                    const int other = w < part ? w : w + 1;
+                    const uint32_t row = handed_at(part, other);
+                    const float2 ml = bars.ml[group * kWarps + other][g];
                     float2 o[kShare];
 #pragma unroll
                     for (int i = 0; i < kShare; ++i) {
-                        o[i] = *reinterpret_cast<const float2*>(row + turned(i) * 8);
+                        o[i] = ld_shared_f2(row ^ (i * 32));
                     }
                     all.join(ml.x, ml.y, o);
                 }
@@ -896,9 +916,19 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                 ++times;
             }
             const int in_group = what.z + group * kHeads + g;
-            if ((which.w == 1 || join_parts(p, all, warp, next.x, which.w, flags & kFirstLater ? 1 : 0)) && in_group < p.group) {
-                write_result<T, D>(p, all, (int64_t)what.x * p.heads + what.y * p.group + in_group, part * kShare * 8);
+            const int64_t row = (int64_t)what.x * p.heads + what.y * p.group + in_group;
+            T* o = in_group < p.group ? static_cast<T*>(p.o) + row * D + part * kShare * 8 : nullptr;
+            float* lse = p.lse && part == 0 ? p.lse + row : nullptr;
+            if (which.w == 1) {
+                if (o) {
+                    write_result(all, o, lse);
+                }
+            } else {
+                const int first_slot = flags & kFirstLater ? 1 : 0, i = (int)blockIdx.x - next.x;
+                write_part(all, p.part_ml, p.part_o, place_of(next.x, first_slot, i) * kHeads + g);
+                join_parts<T, kShare>(p.arrived, p.part_ml, p.part_o, next.x, which.w, first_slot, o, lse);
             }
+            sm.clear();  // (here, so that nothing of the old sums is kept through the above)
             __syncwarp();
         }
         // requests without units: no keys, or lengths that cannot be
@@ -1087,7 +1117,7 @@ extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* s
     }
     const int group = a.heads / c.kv_heads, groups = groups_of(group), blocks = blocks_of(dev->sm_count);
     const Workspace w(blocks, groups, c.head_dim);
-    static_assert(kFan * kFan * kFan * kFan >= kMaxBlocks && kLevels == 4, "levels of joining");
+    static_assert(kFan * kFan * kFan >= kMaxBlocks && kLevels == 3, "levels of joining");
     if (blocks > kMaxBlocks || (int64_t)kLevels * blocks * 2 * kComputeWarps * 4 > SPORK_ATTN_PAGED_COUNTERS) {
         return SPORK_ERR_TOO_LARGE;
     }
