@@ -26,55 +26,56 @@ using namespace spork::ptx;
 // A decoding step is bound by the latency of one dependent chain (lengths, sums, page, slot); a queue of prompts by
 // writing the slot map.
 
-constexpr int kTableThreads = 512;
+constexpr int kTableThreads = 1024;
+constexpr uint32_t kMost = 0x7FFFFFFF;
 
-__device__ __forceinline__ int32_t saturate(int64_t v) { return v > 0x7FFFFFFF ? 0x7FFFFFFF : (int32_t)v; }
+// Sums are kept at 2^31 - 1 once they are beyond it (such sums may be taken in any order), and so fit 32 bits throughout.
+__device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) { return a + b < kMost ? a + b : kMost; }
 
-// Inclusive sum over the block's threads; `total` receives the block's.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t& total)
+// Sum over the threads of the block before this one; `total` receives the block's.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t& total)
 {
+    static_assert(kTableThreads == 32 * 32, "a lane for each warp's sum");
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    auto warp_scan = [&](uint32_t x) {
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const int64_t w = __shfl_up_sync(0xFFFFFFFFu, v, d);
-        v += lane >= d ? w : 0;
-    }
+        for (int d = 1; d < 32; d *= 2) {
+            const uint32_t w = __shfl_up_sync(0xFFFFFFFFu, x, d);
+            x = lane >= d ? plus(x, w) : x;
+        }
+        return x;
+    };
+    v = warp_scan(v);
     if (lane == 31) {
         warp_sums[warp] = v;
     }
     __syncthreads();
-    total = 0;
-    int64_t before = 0;
-#pragma unroll
-    for (int w = 0; w < kTableThreads / 32; ++w) {
-        before += w < warp ? warp_sums[w] : 0;
-        total += warp_sums[w];
-    }
-    return before + v;
+    const uint32_t sums = warp_scan(warp_sums[lane]);
+    total = __shfl_sync(0xFFFFFFFFu, sums, 31);
+    const uint32_t warps = __shfl_sync(0xFFFFFFFFu, sums, warp > 0 ? warp - 1 : 0);
+    const uint32_t lanes = __shfl_up_sync(0xFFFFFFFFu, v, 1);
+    return plus(warp > 0 ? warps : 0, lane > 0 ? lanes : 0);
 }
 
-// What a thread knows of one of its requests, given the tokens of all before it.
-struct Request {
-    int64_t held, adds, need;
-    bool sound;
-    __device__ __forceinline__ Request(const spork_paged_tables_args& a, int r, int64_t tokens_before)
-    {
-        held = a.lengths[r];
-        const int64_t added = a.new_tokens[r];
-        adds = added > 0 ? added : 0;
-        sound = held >= 0 && added >= 0 && (adds == 0 || tokens_before + adds <= a.max_tokens) &&
-                held + adds <= (int64_t)a.max_blocks * a.page_size && held + adds <= 0x7FFFFFFF;
-        need = sound ? (int64_t)pages_of(held + adds, a.page_size) - (int64_t)pages_of(held, a.page_size) : 0;
-    }
+// Tokens to pages: a shift where the page size is a power of two.
+struct Pages {
+    uint32_t size;
+    int shift;  // -1: none
+    __device__ __forceinline__ uint32_t of(uint32_t token) const { return shift >= 0 ? token >> shift : token / size; }
     // of 0 .. 2^31 - 1 tokens
-    static __device__ __forceinline__ uint32_t pages_of(int64_t tokens, uint32_t page)
-    {
-        return ((uint32_t)tokens + page - 1u) / page;
-    }
+    __device__ __forceinline__ uint32_t for_tokens(uint32_t tokens) const { return tokens > 0 ? of(tokens - 1) + 1 : 0; }
+};
+
+// Numbers of the requests in shared memory, one left out after every 32: threads that each walk through requests of their
+// own then meet in no bank, whatever their share.
+struct PerRequest {
+    int32_t* at;
+    __device__ __forceinline__ int32_t& operator[](int r) const { return at[r + (r >> 5)]; }
+    static __host__ __device__ __forceinline__ int space(int requests) { return requests + (requests >> 5); }
 };
 
 // Last of the n ascending entries that is at most v (the first one is).
-__device__ __forceinline__ int last_at_most(const int32_t* entries, int n, int32_t v)
+__device__ __forceinline__ int last_at_most(const PerRequest& entries, int n, int32_t v)
 {
     int low = 0;
     while (n > 1) {
@@ -86,54 +87,76 @@ __device__ __forceinline__ int last_at_most(const int32_t* entries, int n, int32
     return low;
 }
 
-__global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged_tables_args a)
+// kPer: tokens that a thread takes one behind the other.
+template <int kPer>
+__global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged_tables_args a, const Pages page_of)
 {
-    // per request: first token in the slot map, first page among the granted ones, tokens held (-1: refused)
+    // per request: first token in the slot map, first page among the granted ones, tokens held (-1: refused); until those are
+    // known, the tokens that it adds and the pages that it needs (-1: its numbers cannot be)
     extern __shared__ int32_t per_request[];
-    __shared__ int64_t token_sums[kTableThreads / 32], page_sums[kTableThreads / 32];
-    __shared__ int granted_pages, refused;
+    __shared__ uint32_t token_sums[kTableThreads / 32], page_sums[kTableThreads / 32];
+    __shared__ uint32_t granted_pages;
+    __shared__ int refused;
     const int n = a.requests;
-    int32_t *first_token = per_request, *first_page = per_request + n, *held_of = per_request + 2 * n;
+    const int space = PerRequest::space(n);
+    const PerRequest first_token{per_request}, first_page{per_request + space}, held_of{per_request + 2 * space};
     if (threadIdx.x == 0) {
-        granted_pages = refused = 0;
+        granted_pages = 0;
+        refused = 0;
     }
     grid_dependency_wait();
     grid_launch_dependents();
     const int32_t used = *a.free_used;
-    const int64_t left = used >= 0 && used <= a.free_count ? a.free_count - used : 0;
+    const uint32_t left = used >= 0 && used <= a.free_count ? a.free_count - used : 0;
+    for (int r = threadIdx.x; r < n; r += kTableThreads) {
+        held_of[r] = a.lengths[r];
+        first_token[r] = a.new_tokens[r];
+    }
+    __syncthreads();
+    // a thread's requests lie side by side, and nobody else looks at them before the sums are there
     const int chunk = (n + kTableThreads - 1) / kTableThreads;
     const int r0 = (int)threadIdx.x * chunk < n ? (int)threadIdx.x * chunk : n, r1 = r0 + chunk < n ? r0 + chunk : n;
+    const int64_t row_tokens = (int64_t)a.max_blocks * a.page_size;
+    const uint32_t capacity = row_tokens < kMost ? (uint32_t)row_tokens : kMost;
+    const uint32_t room = (uint32_t)a.max_tokens;
 
-    int64_t mine = 0, tokens, pages;
+    uint32_t mine = 0, tokens, pages;
     for (int r = r0; r < r1; ++r) {
-        const int32_t added = a.new_tokens[r];
-        mine += added > 0 ? added : 0;
+        mine = plus(mine, first_token[r] > 0 ? first_token[r] : 0);
     }
-    const int64_t token0 = block_scan(mine, token_sums, tokens) - mine;
-    int64_t token = token0;
+    const uint32_t token0 = block_scan(mine, token_sums, tokens);
+    uint32_t token = token0;
     mine = 0;
     for (int r = r0; r < r1; ++r) {
-        const Request q(a, r, token);
-        token += q.adds;
-        mine += q.need;
+        const int32_t held = held_of[r], added = first_token[r];
+        const uint32_t adds = added > 0 ? added : 0;
+        token = plus(token, adds);
+        const bool sound = held >= 0 && added >= 0 && (adds == 0 || token <= room) && (uint32_t)held + adds <= capacity;
+        const uint32_t need = sound ? page_of.for_tokens(held + adds) - page_of.for_tokens(held) : 0;
+        first_token[r] = adds;
+        first_page[r] = sound ? (int32_t)need : -1;
+        mine = plus(mine, need);
     }
-    int64_t page = block_scan(mine, page_sums, pages) - mine;
+    uint32_t page = block_scan(mine, page_sums, pages);
     token = token0;
-    int most = 0, not_granted = 0;
+    uint32_t most = 0;
+    int not_granted = 0;
     for (int r = r0; r < r1; ++r) {
-        const Request q(a, r, token);
-        const bool granted = q.sound && (q.need == 0 || page + q.need <= left);
-        first_token[r] = saturate(token);
-        first_page[r] = saturate(page);
-        held_of[r] = granted ? (int32_t)q.held : -1;
+        const uint32_t adds = first_token[r], need = first_page[r] > 0 ? first_page[r] : 0;
+        const uint32_t until = plus(page, need);
+        const bool granted = first_page[r] >= 0 && (need == 0 || until <= left);
+        const int32_t held = held_of[r];
+        first_token[r] = (int32_t)token;
+        first_page[r] = (int32_t)page;
+        held_of[r] = granted ? held : -1;
         if (blockIdx.x == 0) {
-            a.offsets[r] = saturate(token);
-            a.lengths_after[r] = (int32_t)(granted ? q.held + q.adds : q.held);
+            a.offsets[r] = (int32_t)token;
+            a.lengths_after[r] = granted ? held + (int32_t)adds : held;
         }
-        token += q.adds;
-        page += q.need;
+        token = plus(token, adds);
+        page = until;
         // what is granted ends where the last granted request with pages does
-        most = granted && q.need > 0 ? (int)page : most;
+        most = granted && need > 0 ? until : most;
         not_granted += granted ? 0 : 1;
     }
     if (most > 0) {
@@ -144,35 +167,60 @@ __global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged
     }
     __syncthreads();
 
-    const int granted = granted_pages;
+    const int granted = (int)granted_pages;
     const int stride = gridDim.x * kTableThreads, at = blockIdx.x * kTableThreads + threadIdx.x;
     if (at == 0) {
-        a.offsets[n] = saturate(tokens);
-        a.info[0] = saturate((int64_t)used + granted);
-        a.info[1] = saturate(tokens);
+        a.offsets[n] = (int32_t)tokens;
+        a.info[0] = used + granted;
+        a.info[1] = (int32_t)tokens;
         a.info[2] = refused;
-        a.info[3] = saturate(pages);
+        a.info[3] = (int32_t)pages;
     }
-    const uint32_t page_size = a.page_size;
     for (int i = at; i < granted; i += stride) {
         const int r = last_at_most(first_page, n, i);
-        const uint32_t old = Request::pages_of(held_of[r], page_size);
+        const uint32_t old = page_of.for_tokens(held_of[r]);
         a.block_table[r * a.table_stride + old + (i - first_page[r])] = a.free_pages[used + i];
     }
-    for (int64_t t = at; t < a.max_tokens; t += stride) {
-        int64_t slot = -1;
-        if (t < tokens) {
-            const int r = last_at_most(first_token, n, (int32_t)t);
-            const int32_t held = held_of[r];
-            if (held >= 0) {
-                const uint32_t place = (uint32_t)held + (uint32_t)(t - first_token[r]);
-                const uint32_t block = place / page_size, old = Request::pages_of(held, page_size);
-                const int32_t of = block < old ? a.block_table[r * a.table_stride + block]
-                                               : a.free_pages[used + first_page[r] + (int)(block - old)];
-                slot = of >= 0 ? (int64_t)of * page_size + (place - block * page_size) : -1;
+    for (int64_t t0 = (int64_t)at * kPer; t0 < a.max_tokens; t0 += (int64_t)stride * kPer) {
+        int64_t slot[kPer];
+        int r = t0 < tokens ? last_at_most(first_token, n, (int32_t)t0) : 0, last_r = -1, of = 0;
+        uint32_t last_block = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int64_t t = t0 + j;
+            slot[j] = -1;
+            if (t < tokens && t < a.max_tokens) {
+                while (j > 0 && r + 1 < n && first_token[r + 1] <= t) {
+                    ++r;
+                }
+                const int32_t held = held_of[r];
+                if (held >= 0) {
+                    const uint32_t place = (uint32_t)held + (uint32_t)(t - first_token[r]);
+                    const uint32_t block = page_of.of(place);
+                    if (kPer == 1 || r != last_r || block != last_block) {
+                        const uint32_t old = page_of.for_tokens(held);
+                        of = block < old ? a.block_table[r * a.table_stride + block]
+                                         : a.free_pages[used + first_page[r] + (int)(block - old)];
+                        last_r = r;
+                        last_block = block;
+                    }
+                    slot[j] = of >= 0 ? (int64_t)of * page_of.size + (place - block * page_of.size) : -1;
+                }
             }
         }
-        a.slots[t] = slot;
+        if (kPer % 2 == 0 && t0 + kPer <= a.max_tokens && (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0) {
+#pragma unroll
+            for (int j = 0; j < kPer / 2; ++j) {
+                reinterpret_cast<longlong2*>(a.slots + t0)[j] = make_longlong2(slot[2 * j], slot[kPer > 1 ? 2 * j + 1 : 0]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                if (t0 + j < a.max_tokens) {
+                    a.slots[t0 + j] = slot[j];
+                }
+            }
+        }
     }
 }
 
@@ -277,24 +325,35 @@ static int launch(void (*kernel)(Params...), unsigned blocks, int threads, size_
     return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-static int launch_tables(const spork_paged_tables_args& a, DeviceState& dev, cudaStream_t stream)
+template <int kPer>
+static int launch_tables(const spork_paged_tables_args& a, DeviceState& dev, unsigned blocks, cudaStream_t stream)
 {
-    const size_t smem = (size_t)a.requests * 3 * sizeof(int32_t);
+    const size_t smem = (size_t)PerRequest::space(a.requests) * 3 * sizeof(int32_t);
     if (smem > 40 * 1024) {  // beyond what a kernel gets unasked (its static arrays included)
         static std::once_flag once[kMaxDevices];
         static cudaError_t err[kMaxDevices];
         std::call_once(once[dev.ordinal], [&] {
-            err[dev.ordinal] = cudaFuncSetAttribute(tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                    SPORK_PAGED_MAX_REQUESTS * 3 * (int)sizeof(int32_t));
+            err[dev.ordinal] = cudaFuncSetAttribute(tables_kernel<kPer>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                    PerRequest::space(SPORK_PAGED_MAX_REQUESTS) * 3 * (int)sizeof(int32_t));
         });
         if (err[dev.ordinal] != cudaSuccess) {
             return (int)err[dev.ordinal];
         }
     }
-    const int64_t wanted = (a.max_tokens + kTableThreads - 1) / kTableThreads;
-    const int64_t most = 2 * (int64_t)dev.sm_count;
-    const unsigned blocks = (unsigned)(wanted < 1 ? 1 : wanted > most ? most : wanted);
-    return launch(tables_kernel, blocks, kTableThreads, smem, stream, a);
+    const uint32_t size = (uint32_t)a.page_size;
+    return launch(tables_kernel<kPer>, blocks, kTableThreads, smem, stream, a,
+                  Pages{size, (size & (size - 1)) == 0 ? __builtin_ctz(size) : -1});
+}
+
+static int launch_tables(const spork_paged_tables_args& a, DeviceState& dev, cudaStream_t stream)
+{
+    // One token to a thread while a block on every SM holds them all: the page numbers of decoding requests are then
+    // looked up side by side.  Beyond that four, which mostly are one request's and in one page.
+    const int64_t most = dev.sm_count, wanted = (a.max_tokens + kTableThreads - 1) / kTableThreads;
+    if (wanted <= most) {
+        return launch_tables<1>(a, dev, (unsigned)(wanted < 1 ? 1 : wanted), stream);
+    }
+    return launch_tables<4>(a, dev, (unsigned)(wanted < 4 * most ? (wanted + 3) / 4 : most), stream);
 }
 
 template <typename Src, typename Dst, int kElems>
@@ -358,7 +417,7 @@ extern "C" int spork_paged_sm100_tables(const spork_paged_tables_args* args, voi
         (a.requests > 1 && a.table_stride < a.max_blocks)) {
         return SPORK_ERR_UNSUPPORTED_SHAPE;
     }
-    if (a.requests > SPORK_PAGED_MAX_REQUESTS || a.max_tokens > 0x7FFFFFFF) {
+    if (a.requests > SPORK_PAGED_MAX_REQUESTS || a.max_tokens >= 0x7FFFFFFF || a.free_count == 0x7FFFFFFF) {
         return SPORK_ERR_TOO_LARGE;
     }
     struct Span {

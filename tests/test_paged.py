@@ -37,7 +37,7 @@ def attn_args(c=None, **kw):
 @pytest.mark.parametrize("change,code", [
     (dict(requests=-1), 10002), (dict(page_size=0), 10002), (dict(max_tokens=-1), 10002), (dict(table_stride=7), 10002),
     (dict(free_count=-1), 10002), (dict(max_blocks=-1), 10002), (dict(requests=16385, table_stride=8), 10006),
-    (dict(max_tokens=1 << 31), 10006), (dict(lengths=0), 10001), (dict(slots=FAKE + 5 * 4096 + 4), 10001),
+    (dict(max_tokens=(1 << 31) - 1), 10006), (dict(free_count=(1 << 31) - 1), 10006), (dict(lengths=0), 10001), (dict(slots=FAKE + 5 * 4096 + 4), 10001),
     (dict(lengths_after=FAKE), 10001), (dict(lengths_after=FAKE + 12), 10001), (dict(info=FAKE + 4 * 4096), 10001),
     (dict(offsets=FAKE + 5 * 4096 + 64), 10001), (dict(free_pages=FAKE + 2 * 4096 + 64), 10001), (dict(info=FAKE + 2), 10001)])
 def test_tables_refuses(sp, change, code):
