@@ -110,8 +110,8 @@ struct alignas(16) Note {
     int parts, first;        // the blocks that have units of this (request, key head): how many, and the first one
     int next_r, next_kv, next_head;  // with the last of the block's units: what comes next (-1: nothing)
 };
-// the run's end; this part is a later one of its block's (Walk::later); so is the first part; a bad page
-constexpr int kDone = 1, kLater = 2, kFirstLater = 4, kBad = 8;
+// nothing more; the first part is a later one of its block's (is_later); a bad page
+constexpr int kDone = 1, kFirstLater = 2, kBad = 4;
 
 struct Bars {
     uint64_t full[4], empty[4];
@@ -699,8 +699,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                     const uint32_t first_block = cut.at(walk.base);
                     plan.note.first = (int)first_block;
                     plan.note.parts = (int)(cut.at(walk.base + walk.units - 1) - first_block) + 1;
-                    plan.note.flags = (is_later(from, walk.base) ? kLater : 0) |
-                                      (is_later(cut.begin(first_block), walk.base) ? kFirstLater : 0);
+                    plan.note.flags = is_later(cut.begin(first_block), walk.base) ? kFirstLater : 0;
                 }
                 more = settle(walk.next(p, length));
                 unit = walk.first;
