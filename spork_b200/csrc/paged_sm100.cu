@@ -105,7 +105,6 @@ __global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged
         refused = 0;
     }
     grid_dependency_wait();
-    grid_launch_dependents();
     const int32_t used = *a.free_used;
     const uint32_t left = used >= 0 && used <= a.free_count ? a.free_count - used : 0;
     for (int r = threadIdx.x; r < n; r += kTableThreads) {
@@ -167,6 +166,9 @@ __global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged
     }
     __syncthreads();
 
+    // (not at the begin: blocks of the next launch that come so early slow the sums down, 16.4 us instead of 10.6 for the maps
+    // of 2048 prompts in a stream of such launches; at the end it was 13.0)
+    grid_launch_dependents();
     const int granted = (int)granted_pages;
     const int stride = gridDim.x * kTableThreads, at = blockIdx.x * kTableThreads + threadIdx.x;
     if (at == 0) {
