@@ -464,6 +464,15 @@ int spork_attn_sm100_paged_supports(int heads, int kv_heads, int head_dim, int p
 /* Bytes of workspace on the current device; negative: minus an error code. */
 int64_t spork_attn_sm100_paged_workspace(int heads, int kv_heads, int head_dim);
 int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* stream);
+/* Host-only view of how a launch is laid out (no CUDA call; usable without a GPU): what
+ * block `block` of one on sm_count SMs works on, given the lengths in HOST memory.
+ * Nine words for each run of units: request, key head, unit of its query heads, first
+ * unit of keys, units here, units in all, and, where they are not all here, the first
+ * block that has some, the number of blocks that do, and this block's slot (0 / 1) in
+ * the workspace.  Returns their number (those beyond `capacity` are not written), or
+ * -1 on bad arguments. */
+int spork_attn_sm100_paged_plan(const int32_t* lengths, int requests, int heads, int kv_heads, int head_dim, int page_size,
+                                int max_blocks, int sm_count, int block, int32_t* out, int capacity);
 
 /* Library/build information: "spork_b200 <version> sm_100a". */
 const char* spork_b200_version(void);

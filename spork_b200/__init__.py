@@ -19,6 +19,7 @@ from .api import (  # noqa: F401
     SporkError,
     attn_fwd,
     attn_paged,
+    attn_paged_plan,
     attn_paged_supports,
     attn_paged_workspace,
     choice,

@@ -127,6 +127,8 @@ def lib() -> ctypes.CDLL:
         L.spork_attn_sm100_paged_supports.restype = i32
         L.spork_attn_sm100_paged_workspace.argtypes = [i32, i32, i32]
         L.spork_attn_sm100_paged_workspace.restype = ctypes.c_int64
+        L.spork_attn_sm100_paged_plan.argtypes = [ctypes.POINTER(i32)] + [i32] * 8 + [ctypes.POINTER(i32), i32]
+        L.spork_attn_sm100_paged_plan.restype = i32
         L.spork_b200_version.restype = ctypes.c_char_p
         _lib = L
     return _lib
@@ -686,6 +688,22 @@ def attn_paged_workspace(heads: int, kv_heads: int, head_dim: int) -> int:
     if n < 0:
         raise SporkError(-n, "spork_attn_sm100_paged_workspace")
     return n
+
+
+def attn_paged_plan(lengths, block: int, *, heads: int, kv_heads: int, head_dim: int, page_size: int, max_blocks: int,
+                    sm_count: int = 148) -> list[dict]:
+    """What one block of an attn_paged launch works on, for lengths known on the host (a sequence of ints); computed without
+    a GPU (spork_attn_sm100_paged_plan)."""
+    n = len(lengths)
+    host = (ctypes.c_int * max(n, 1))(*lengths)
+    args = (host, n, heads, kv_heads, head_dim, page_size, max_blocks, sm_count, block)
+    count = lib().spork_attn_sm100_paged_plan(*args, None, 0)
+    if count < 0:
+        raise ValueError("not a launch that attn_paged makes")
+    out = (ctypes.c_int * max(9 * count, 1))()
+    lib().spork_attn_sm100_paged_plan(*args, out, count)
+    keys = ("request", "kv_head", "head_unit", "first", "count", "units", "first_block", "blocks", "slot")
+    return [dict(zip(keys, out[9 * i:9 * i + 9])) for i in range(count)]
 
 
 def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, scale: float | None = None, workspace=None,

@@ -127,7 +127,7 @@ static_assert(kBlocksPerSm * (Config<128, 1>::kSmem + (int)sizeof(Bars) + 1024) 
 
 // Units of a request: none if there is nothing to read, or nothing that may be read.
 template <int kTile>
-__device__ __forceinline__ int units_of(const Params& p, int len)
+__host__ __device__ __forceinline__ int units_of(const Params& p, int len)
 {
     return len > 0 && len <= p.capacity ? (int)(((uint32_t)len + kTile - 1) / kTile) : 0;
 }
@@ -136,15 +136,15 @@ __device__ __forceinline__ int units_of(const Params& p, int len)
 // fewer than 2^31 places.)
 struct Cut {
     uint32_t total, blocks, each, rest;
-    __device__ __forceinline__ Cut(uint32_t places, uint32_t grid)
+    __host__ __device__ __forceinline__ Cut(uint32_t places, uint32_t grid)
         : total(places), blocks(places < grid * kMinRun ? (places + kMinRun - 1) / kMinRun : grid)
     {
         each = blocks ? total / blocks : 0;
         rest = total - each * blocks;
     }
-    __device__ __forceinline__ uint32_t begin(uint32_t b) const { return b * each + b * rest / blocks; }
+    __host__ __device__ __forceinline__ uint32_t begin(uint32_t b) const { return b * each + b * rest / blocks; }
     // the block whose run has a place
-    __device__ __forceinline__ uint32_t at(uint32_t place) const
+    __host__ __device__ __forceinline__ uint32_t at(uint32_t place) const
     {
         return (uint32_t)(((uint64_t)(place + 1) * blocks - 1) / total);
     }
@@ -157,7 +157,7 @@ struct Walk {
     int r, kv, hu, first, count, units, len;
     uint32_t base, from, end;  // places in the list: of the current one's first unit, of the run's begin and end
 
-    __device__ __forceinline__ void here()
+    __host__ __device__ __forceinline__ void here()
     {
         if (units <= kWhole) {
             const uint32_t middle = base + units / 2;
@@ -170,8 +170,9 @@ struct Walk {
         }
     }
     // to the next one; false at the run's end
+#pragma nv_exec_check_disable
     template <typename Length>
-    __device__ __forceinline__ bool next(const Params& p, const Length& length)
+    __host__ __device__ __forceinline__ bool next(const Params& p, const Length& length)
     {
         base += units + kPairCost;
         if (base >= end) {
@@ -197,7 +198,7 @@ struct Walk {
 
 // Where a block's part of a (request, head unit) goes in the workspace: a run that begins in front of it (and of its
 // predecessor's cost) has other units first, and at its begin it may have a part of those.
-__device__ __forceinline__ bool is_later(uint32_t from, uint32_t base) { return from + kPairCost < base; }
+__host__ __device__ __forceinline__ bool is_later(uint32_t from, uint32_t base) { return from + kPairCost < base; }
 
 __device__ __forceinline__ float ex2(float x)
 {
@@ -992,6 +993,22 @@ static int make_map(CUtensorMap* map, void* base, const spork_paged_cache& c, co
     return r == CUDA_SUCCESS ? 0 : SPORK_ERR_DRIVER;
 }
 
+// What the list of units depends on besides the lengths.
+static int fill_shape(Params& p, int requests, int heads, int kv_heads, int head_dim, int page_size, int max_blocks)
+{
+    const int group = heads / kv_heads, unit_heads = groups_of(group) * kHeads;
+    p.requests = requests;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.group = group;
+    p.head_units = (group + unit_heads - 1) / unit_heads;
+    const int64_t capacity = (int64_t)max_blocks * page_size;
+    p.capacity = capacity < 0x7FFFFFFF ? (int32_t)capacity : 0x7FFFFFFF;
+    // places in the list, at most
+    const int64_t places = (p.capacity / (8192 / head_dim) + 1 + kPairCost) * (int64_t)requests * kv_heads * p.head_units;
+    return places < 0x7FFFFFFF ? 0 : SPORK_ERR_TOO_LARGE;
+}
+
 struct Workspace {
     int64_t ml, o, bytes;
     Workspace(int blocks, int groups, int D)
@@ -1048,6 +1065,81 @@ static int launch_q(bool f32, int groups, const CUtensorMap& map_k, const CUtens
 
 }  // namespace attn_paged_sm100
 }  // namespace spork
+
+namespace spork {
+namespace attn_paged_sm100 {
+
+// What block `block` of a launch on sm_count SMs works on, as the kernel finds it.
+template <int kTile>
+static int plan(const Params& p, const int32_t* lengths, uint32_t grid, uint32_t block, int32_t* out, int capacity)
+{
+    const auto length = [&](int r) { return lengths[r]; };
+    const int hhs = p.kv_heads * p.head_units;
+    uint32_t places = 0;
+    const auto places_of = [&](int r) {
+        const int units = units_of<kTile>(p, lengths[r]);
+        return units ? (uint32_t)(units + kPairCost) * hhs : 0u;
+    };
+    for (int r = 0; r < p.requests; ++r) {
+        places += places_of(r);
+    }
+    const Cut cut(places, grid);
+    if (block >= cut.blocks) {
+        return 0;
+    }
+    Walk<kTile> walk{};
+    walk.from = cut.begin(block);
+    walk.end = cut.begin(block + 1);
+    while (walk.from - walk.base >= places_of(walk.r)) {
+        walk.base += places_of(walk.r++);
+    }
+    walk.len = lengths[walk.r];
+    walk.units = units_of<kTile>(p, walk.len);
+    const uint32_t each = walk.units + kPairCost, hh = (walk.from - walk.base) / each;
+    walk.base += hh * each;
+    walk.kv = hh / p.head_units;
+    walk.hu = hh % p.head_units;
+    walk.here();
+    int n = 0;
+    do {
+        if (walk.count == 0) {
+            continue;
+        }
+        if (n < capacity) {
+            const bool whole = walk.count == walk.units;
+            const int first = whole ? (int)block : (int)cut.at(walk.base);
+            const int32_t row[9] = {walk.r, walk.kv, walk.hu, walk.first, walk.count, walk.units, first,
+                                    whole ? 1 : (int)cut.at(walk.base + walk.units - 1) - first + 1,
+                                    !whole && is_later(cut.begin(block), walk.base) ? 1 : 0};
+            for (int i = 0; i < 9; ++i) {
+                out[n * 9 + i] = row[i];
+            }
+        }
+        ++n;
+    } while (walk.next(p, length));
+    return n;
+}
+
+}  // namespace attn_paged_sm100
+}  // namespace spork
+
+extern "C" int spork_attn_sm100_paged_plan(const int32_t* lengths, int requests, int heads, int kv_heads, int head_dim,
+                                           int page_size, int max_blocks, int sm_count, int block, int32_t* out, int capacity)
+{
+    using namespace spork::attn_paged_sm100;
+    if (!spork_attn_sm100_paged_supports(heads, kv_heads, head_dim, page_size) || heads == 0 || requests < 0 || max_blocks < 0 ||
+        (requests > 0 && !lengths) || sm_count < 1 || block < 0 || block >= blocks_of(sm_count) || capacity < 0 ||
+        (capacity > 0 && !out)) {
+        return -1;
+    }
+    Params p{};
+    if (fill_shape(p, requests, heads, kv_heads, head_dim, page_size, max_blocks) != 0) {
+        return -1;
+    }
+    const uint32_t grid = (uint32_t)blocks_of(sm_count);
+    return head_dim == 128 ? plan<64>(p, lengths, grid, (uint32_t)block, out, capacity)
+                           : plan<128>(p, lengths, grid, (uint32_t)block, out, capacity);
+}
 
 extern "C" int spork_attn_sm100_paged_supports(int heads, int kv_heads, int head_dim, int page_size)
 {
@@ -1138,16 +1230,9 @@ extern "C" int spork_attn_sm100_paged(const spork_attn_paged_args* args, void* s
     p.q_request_stride = a.q_request_stride;
     p.q_head_stride = a.q_head_stride;
     p.table_stride = a.table_stride;
-    p.requests = a.requests;
-    p.heads = a.heads;
-    p.kv_heads = c.kv_heads;
-    p.group = group;
-    p.head_units = (group + groups * kHeads - 1) / (groups * kHeads);
-    const int64_t capacity = (int64_t)a.max_blocks * c.page_size;
-    p.capacity = capacity < 0x7FFFFFFF ? (int32_t)capacity : 0x7FFFFFFF;
-    // places in the list of units, at most
-    if (((p.capacity >> 6) + 1 + kPairCost) * (int64_t)a.requests * c.kv_heads * p.head_units > 0x7FFFFFFF) {
-        return SPORK_ERR_TOO_LARGE;
+    const int rc4 = fill_shape(p, a.requests, a.heads, c.kv_heads, c.head_dim, c.page_size, a.max_blocks);
+    if (rc4) {
+        return rc4;
     }
     p.num_pages = c.num_pages;
     p.page_size = c.page_size;

@@ -145,3 +145,71 @@ def test_wrappers_refuse_shapes_types_and_host_tensors(sp):
                dict(o=q)):
         with pytest.raises(TypeError):
             attn(**kw)
+
+
+# ------------------------------------------------------------------------------------------------ how a launch is cut
+
+def _plan(sp, lengths, **kw):
+    args = dict(heads=8, kv_heads=2, head_dim=128, page_size=16, max_blocks=1 << 14, sm_count=148) | kw
+    return [sp.attn_paged_plan(lengths, b, **args) for b in range(2 * args["sm_count"])], args
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_every_unit_is_in_one_run_and_every_part_has_a_place(sp, seed):
+    """The kernel's own cutting, on the host: all units of each (request, key head, unit of query heads) once, in the order
+    of the blocks; the parts of one that is cut are those of neighbouring blocks, each in a slot of its own, the first one
+    in the slot that the others' joining computes for it and all others in slot 0; short ones are not cut; runs are of one
+    size."""
+    import random
+
+    rng = random.Random(seed)
+    dim = rng.choice([64, 128])
+    tile = 8192 // dim
+    kv_heads, group = rng.choice([(1, 1), (2, 5), (8, 8), (4, 16), (1, 71), (3, 33)])
+    most = rng.choice([1, 3, 40, 700, 5000, 100000])
+    lengths = [rng.choice([0, 1, tile, tile + 1, rng.randint(0, most), -3, 1 << 30]) for _ in range(rng.choice([1, 2, 23, 300, 1000]))]
+    blocks, args = _plan(sp, lengths, heads=kv_heads * group, kv_heads=kv_heads, head_dim=dim, sm_count=rng.choice([148, 3, 64]))
+    capacity = args["max_blocks"] * args["page_size"]
+    head_units = -(-group // (8 if group <= 8 else 16 if group <= 16 else 32))
+    found, slots = {}, set()
+    for b, runs in enumerate(blocks):
+        for run in runs:
+            found.setdefault((run["request"], run["kv_head"], run["head_unit"]), []).append((b, run))
+    want = {(r, kv, hu): -(-n // tile) for r, n in enumerate(lengths) if 0 < n <= capacity
+            for kv in range(kv_heads) for hu in range(head_units)}
+    assert set(found) == set(want)
+    for key, parts in found.items():
+        at = 0
+        for i, (b, run) in enumerate(parts):
+            assert run["first"] == at and run["units"] == want[key] and run["count"] > 0
+            at += run["count"]
+            if len(parts) > 1:
+                assert run["blocks"] == len(parts) and run["first_block"] + i == b
+                assert i == 0 or run["slot"] == 0
+                assert (b, run["slot"]) not in slots
+                slots.add((b, run["slot"]))
+        assert at == want[key]
+        assert len(parts) == 1 or want[key] > 4
+    # a run: its units and what a (request, head unit) costs besides, one unit; those that are not cut lie to either side
+    sizes = [sum(run["count"] + 1 for run in runs) for runs in blocks]
+    total = sum(n + 1 for n in want.values())
+    assert max(sizes, default=0) <= -(-total // len(blocks)) + 2 + 2 * 5
+
+
+def test_small_launches_are_not_cut_into_crumbs(sp):
+    blocks, _ = _plan(sp, [64 * 6])
+    busy = [runs for runs in blocks if runs]
+    assert len(busy) <= 8 and all(sum(r["count"] for r in runs) >= 1 for runs in busy)
+    blocks, _ = _plan(sp, [64 * 4, 1, 100], heads=2)
+    assert all(run["count"] == run["units"] for runs in blocks for run in runs)
+
+
+def test_plan_refuses(sp):
+    for kw in (dict(heads=7), dict(head_dim=96), dict(page_size=24), dict(sm_count=0), dict(max_blocks=-1)):
+        with pytest.raises(ValueError):
+            sp.attn_paged_plan([100], 0, **(dict(heads=8, kv_heads=2, head_dim=128, page_size=16, max_blocks=64) | kw))
+    with pytest.raises(ValueError):
+        sp.attn_paged_plan([100], 296, heads=8, kv_heads=2, head_dim=128, page_size=16, max_blocks=64)
+    # more places in the list than 32 bits number: 2^25 units a request
+    with pytest.raises(ValueError):
+        sp.attn_paged_plan([100] * 100, 0, heads=8, kv_heads=2, head_dim=128, page_size=64, max_blocks=1 << 25)

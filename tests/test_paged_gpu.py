@@ -277,6 +277,29 @@ def test_attention_of_one_long_request(sp, cuda, keys, heads, kv_heads, dim, pag
         case.kc[page_id, :, at % page], case.k[0] = was, old
 
 
+@pytest.mark.parametrize("seed", range(16))
+def test_attention_of_drawn_shapes(sp, cuda, seed):
+    import torch
+
+    rng = random.Random(seed)
+    dim, page = rng.choice([64, 128]), rng.choice([8, 16, 32, 64, 128, 320])
+    kv_heads, group = rng.choice([(1, 3), (2, 8), (3, 9), (4, 1), (1, 17), (2, 30), (1, 40), (8, 4)])
+    most = rng.choice([70, 600, 2500])
+    lengths = [rng.choice([0, 1, rng.randint(0, most)]) for _ in range(rng.choice([1, 3, 17, 90]))]
+    dtype = rng.choice([torch.float16, torch.bfloat16])
+    case = Paged(cuda, lengths, kv_heads * group, kv_heads, dim, page, dtype, rng.choice([None, torch.float32]),
+                 rng.choice(["heads", "tokens", "both", "wide"]), seed=seed, width=rng.choice([None, 1 + -(-most // page) + 40]))
+    case.check(*case.run(sp))
+
+
+def test_attention_of_more_requests_than_a_block_keeps_lengths_of(sp, cuda):
+    import torch
+
+    rng = random.Random(3)
+    case = Paged(cuda, [rng.choice([0, 1, 130, 400]) for _ in range(1100)], 4, 1, 64, 64, torch.float16, seed=5)
+    case.check(*case.run(sp))
+
+
 def test_attention_large_scores_and_small_weights(sp, cuda):
     """Scores of several hundred: all but a few weights vanish, nothing overflows."""
     import torch
@@ -423,6 +446,17 @@ def test_another_stream_and_the_wrong_device(sp, cuda):
                        torch.zeros(900, dtype=torch.int64))
 
 
+def test_launches_of_other_shapes_share_a_streams_workspace(sp, cuda):
+    """The kept workspace grows with what a launch needs, and every launch leaves its counters at zero for the next one."""
+    import torch
+
+    cases = [Paged(cuda, [2000, 5, 700], h, kv, d, 16, torch.float16, seed=h) for h, kv, d in
+             ((4, 4, 64), (32, 1, 128), (16, 2, 64), (8, 8, 128), (71, 1, 128))]
+    for _ in range(3):
+        for c in cases:
+            c.check(*c.run(sp))
+
+
 def test_two_streams_at_once(sp, cuda):
     """Calls that overlap have workspaces of their own."""
     import torch
@@ -465,6 +499,24 @@ def test_captured_graphs_follow_the_lengths(sp, cuda):
         torch.cuda.synchronize()
         for w, o in zip(want, outs):
             assert torch.equal(w, o)
+
+
+def test_the_range_checked_build_agrees(sp, cuda):
+    """Every kernel through libspork_b200_checked.so, in a process of its own: no range check fires, results are right."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    checked = os.path.join(root, "spork_b200", "libspork_b200_checked.so")
+    if not os.path.exists(checked):
+        pytest.skip("libspork_b200_checked.so was not built (python -m spork_b200.build --checked)")
+    if os.environ.get("SPORK_B200_LIBRARY") == checked:
+        pytest.skip("this is that process")
+    names = "attention_matches or many_requests or one_long or bad_pages or captured or test_store or tables_match"
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-k", names, os.path.abspath(__file__)],
+                       capture_output=True, text=True, env=dict(os.environ, SPORK_B200_LIBRARY=checked), timeout=600, cwd=root)
+    assert r.returncode == 0 and "passed" in r.stdout, r.stdout[-3000:] + r.stderr[-2000:]
 
 
 # ------------------------------------------------------------------------------------------------ all together
