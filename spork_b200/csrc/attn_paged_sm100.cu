@@ -97,7 +97,7 @@ struct Params {
     // workspace
     uint32_t* arrived; // [level][block][slot][warp]: parts that are there, of those whose first one is that; zero between calls
     float2* part_ml;   // [block][slot][warp][head]: maximum, sum
-    float* part_o;     // [block][slot][warp][head][the warp's share of D]
+    float* part_o;     // [block][slot][warp][lane][the lane's columns of the warp's share of D]
     uint32_t* status;
 };
 
@@ -431,16 +431,33 @@ struct Part {
         l = 0.0f;
     }
 
-    __device__ __forceinline__ void join(float its_m, float its_l, const float2 (&its_o)[kShare])
+    // With others, in order: one common maximum, so that the weights do not wait for one another.  (One that is not there has
+    // the maximum -infinity, the sum 0 and an output of 0.)
+    template <int kMost>
+    __device__ __forceinline__ void join(const float2 (&ml)[kMost], const float2 (&its_o)[kMost][kShare])
     {
-        const float most = fmaxf(m, its_m), to = most == -INFINITY ? 0.0f : most;
-        const float down = ex2(m - to), its_down = ex2(its_m - to);
-        l = l * down + its_l * its_down;
-        m = most;
+        float most = m;
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) {
+            most = fmaxf(most, ml[j].x);
+        }
+        const float to = most == -INFINITY ? 0.0f : most, down = ex2(m - to);
+        l *= down;
 #pragma unroll
         for (int i = 0; i < kShare; ++i) {
-            o[i].x = o[i].x * down + its_o[i].x * its_down;
-            o[i].y = o[i].y * down + its_o[i].y * its_down;
+            o[i].x *= down;
+            o[i].y *= down;
+        }
+        m = most;
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) {
+            const float its = ex2(ml[j].x - to);
+            l += ml[j].y * its;
+#pragma unroll
+            for (int i = 0; i < kShare; ++i) {
+                o[i].x += its_o[j][i].x * its;
+                o[i].y += its_o[j][i].y * its;
+            }
         }
     }
 };
@@ -461,18 +478,48 @@ __device__ __forceinline__ void write_result(const Part<kShare>& all, T* o, floa
     }
 }
 
-// A part in the workspace: [warp][head], maxima and sums, and [warp][head][the warp's share of D].
+// A part in the workspace: maxima and sums by head, and each lane's columns side by side.
 template <int kShare>
-__device__ __forceinline__ void write_part(const Part<kShare>& all, float2* part_ml, float* part_o, uint32_t row)
+__device__ __forceinline__ void write_part(const Part<kShare>& all, float2* part_ml, float* part_o, uint32_t place)
 {
-    const int t = threadIdx.x % 4;
-    float* out = part_o + row * (kShare * 8) + 2 * t;
+    const int lane = threadIdx.x % 32;
+    float4* out = reinterpret_cast<float4*>(part_o) + (place * 32 + lane) * (kShare / 2);
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-        __stcg(reinterpret_cast<float2*>(out + i * 8), all.o[i]);
+    for (int i = 0; i < kShare / 2; ++i) {
+        __stcg(out + i, make_float4(all.o[2 * i].x, all.o[2 * i].y, all.o[2 * i + 1].x, all.o[2 * i + 1].y));
     }
-    if (t == 0) {
-        __stcg(part_ml + row, make_float2(all.m, all.l));
+    if (lane % 4 == 0) {
+        __stcg(part_ml + place * kHeads + lane / 4, make_float2(all.m, all.l));
+    }
+}
+
+// (Predicated, not branched around: with branches the compiler keeps more registers than there are.)
+template <int kShare>
+__device__ __forceinline__ void read_part(float2& ml, float2 (&o)[kShare], const float2* part_ml, const float* part_o,
+                                          uint32_t place, bool there)
+{
+    const int lane = threadIdx.x % 32;
+    const float4* from = reinterpret_cast<const float4*>(part_o) + (place * 32 + lane) * (kShare / 2);
+    ml = make_float2(-INFINITY, 0.0f);
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %3, 0;\n\t"
+        "@p ld.global.cg.v2.f32 {%0, %1}, [%2];\n\t"
+        "}"
+        : "+f"(ml.x), "+f"(ml.y)
+        : "l"(part_ml + place * kHeads + lane / 4), "r"((int)there));
+#pragma unroll
+    for (int i = 0; i < kShare; i += 2) {
+        o[i] = o[i + 1] = make_float2(0.0f, 0.0f);
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %5, 0;\n\t"
+            "@p ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n\t"
+            "}"
+            : "+f"(o[i].x), "+f"(o[i].y), "+f"(o[i + 1].x), "+f"(o[i + 1].y)
+            : "l"(from + i / 2), "r"((int)there));
     }
 }
 
@@ -491,7 +538,7 @@ template <typename T, int kShare>
 __device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, float* part_o, int first, int parts, int first_slot,
                                         T* o, float* lse)
 {
-    const int lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const int lane = threadIdx.x % 32;
     int mine = (int)blockIdx.x - first, step = 1;  // part i of a level is where part i * step of the lowest one was
     for (int n = parts; n > 1; n = (n + kFan - 1) / kFan, step *= kFan, mine /= kFan) {
         const int begin = mine / kFan * kFan, members = n - begin < kFan ? n - begin : kFan;
@@ -513,26 +560,14 @@ __device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, f
             }
             Part<kShare> all;
             all.clear();
-            constexpr int kAtOnce = kShare <= 4 ? 2 : 1;
+            constexpr int kAtOnce = kShare <= 4 ? 8 : kShare == 8 ? 4 : 2;
             for (int k = 0; k < members; k += kAtOnce) {
                 float2 ml[kAtOnce], x[kAtOnce][kShare];
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
-                    if (j == 0 || k + j < members) {
-                        const uint32_t row = place_of(first, first_slot, (begin + k + j) * step) * kHeads + g;
-                        ml[j] = __ldcg(part_ml + row);
-#pragma unroll
-                        for (int i = 0; i < kShare; ++i) {
-                            x[j][i] = __ldcg(reinterpret_cast<const float2*>(part_o + row * (kShare * 8) + 2 * t + i * 8));
-                        }
-                    }
+                    read_part(ml[j], x[j], part_ml, part_o, place_of(first, first_slot, (begin + k + j) * step), k + j < members);
                 }
-#pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    if (j == 0 || k + j < members) {
-                        all.join(ml[j].x, ml[j].y, x[j]);
-                    }
-                }
+                all.join(ml, x);
             }
             if (n <= kFan) {
                 if (o) {
@@ -540,7 +575,7 @@ __device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, f
                 }
                 return;
             }
-            write_part(all, part_ml, part_o, place_of(first, first_slot, begin * step) * kHeads + g);
+            write_part(all, part_ml, part_o, place_of(first, first_slot, begin * step));
         }
         arrived += gridDim.x * 2 * kComputeWarps;  // (one alone is its own join, where it is)
     }
@@ -885,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                     }
                 }
             }
-            if (kWarps > 1) {
+            if constexpr (kWarps > 1) {
                 if (t == 0) {
                     bars.ml[warp][g] = make_float2(sm.m, l);
                 }
@@ -897,18 +932,18 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                 if (!ok) {
                     break;
                 }
+                float2 ml[kWarps - 1], o[kWarps - 1][kShare];
 #pragma unroll
                 for (int w = 0; w < kWarps - 1; ++w) {
                     const int other = w < part ? w : w + 1;
                     const uint32_t row = handed_at(part, other);
-                    const float2 ml = bars.ml[group * kWarps + other][g];
-                    float2 o[kShare];
+                    ml[w] = bars.ml[group * kWarps + other][g];
 #pragma unroll
                     for (int i = 0; i < kShare; ++i) {
-                        o[i] = ld_shared_f2(row ^ (i * 32));
+                        o[w][i] = ld_shared_f2(row ^ (i * 32));
                     }
-                    all.join(ml.x, ml.y, o);
                 }
+                all.join(ml, o);
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(smem_u32(&bars.taken[group]));
@@ -925,7 +960,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                 }
             } else {
                 const int first_slot = flags & kFirstLater ? 1 : 0, i = (int)blockIdx.x - next.x;
-                write_part(all, p.part_ml, p.part_o, place_of(next.x, first_slot, i) * kHeads + g);
+                write_part(all, p.part_ml, p.part_o, place_of(next.x, first_slot, i));
                 join_parts<T, kShare>(p.arrived, p.part_ml, p.part_o, next.x, which.w, first_slot, o, lse);
             }
             sm.clear();  // (here, so that nothing of the old sums is kept through the above)
