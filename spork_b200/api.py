@@ -473,6 +473,7 @@ _PAGED_ATTN_ARGS = struct.Struct("=" + _CACHE + "6Q4q4ifi")
 # kernels of a few microseconds, so they look each property of a tensor up once and call as little as they can
 _T = None
 _TYPE_CODES: dict = {}
+_CACHE_TYPES: set = set()
 _current_device = _raw_stream = _capturing = None
 _workspace_bytes: dict = {}  # by device and what the size depends on
 _workspaces: dict = {}       # by device and stream: the one that calls without a workspace of their own use
@@ -484,6 +485,7 @@ def _bind_torch():
     import torch
 
     _TYPE_CODES.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    _CACHE_TYPES.update((torch.float16, torch.bfloat16))
     _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     _capturing = torch._C._cuda_isCurrentStreamCapturing
     _T = torch
@@ -706,6 +708,38 @@ def attn_paged_plan(lengths, block: int, *, heads: int, kv_heads: int, head_dim:
     return [dict(zip(keys, out[9 * i:9 * i + 9])) for i in range(count)]
 
 
+def _refuse_attn_paged(q, k_cache, v_cache, block_table, lengths, o, lse):
+    """Raise for what is wrong with the tensors of an attn_paged call."""
+    q_shape = q.shape
+    if len(q_shape) != 3:
+        raise ValueError(f"q must be (R, heads, head_dim), got {tuple(q_shape)}")
+    n, heads, dim = q_shape
+    shape, code, _, _ = _pages(k_cache, v_cache)
+    if shape[3] != dim:
+        raise ValueError(f"q has head dimension {dim}, the cache {shape[3]}")
+    if _TYPE_CODES.get(q.dtype) not in (2, code):
+        raise TypeError(f"q must be float32 or of the cache's type {k_cache.dtype}, got {q.dtype}")
+    if q.stride()[2] != 1:
+        raise ValueError("the head dimension of q must be contiguous")
+    _block_table(block_table, n)
+    _vector(lengths, n, _T.int32, "lengths")
+    if o is not None:
+        if o.shape != q_shape:
+            raise ValueError(f"o must have q's shape {(n, heads, dim)}, got {tuple(o.shape)}")
+        if o.dtype is not k_cache.dtype:
+            raise TypeError(f"o must be of the cache's type {k_cache.dtype}, got {o.dtype}")
+        if not o.is_contiguous():
+            raise ValueError("o must be contiguous")
+    if lse is not None:
+        if lse.shape != (n, heads) or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous ({n}, {heads}), got {tuple(lse.shape)}")
+        if lse.dtype is not _T.float32:
+            raise TypeError(f"lse must be torch.float32, got {lse.dtype}")
+    _on_gpu(q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths,
+            **{name: t for name, t in (("o", o), ("lse", lse)) if t is not None})
+    raise ValueError("q, the cache and the block table do not fit together")
+
+
 def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, scale: float | None = None, workspace=None,
                stream=None):
     """o[r] = softmax(scale q[r] K^T) V over the first ``lengths[r]`` keys that request r holds in the cache.
@@ -720,42 +754,30 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     the same time (other streams, other captured graphs) need one each.  Without one, a stream's launches share one that is
     kept for the stream, and a captured launch gets its own."""
     torch = _T or _bind_torch()
-    q_shape = q.shape
-    if len(q_shape) != 3:
-        raise ValueError(f"q must be (R, heads, head_dim), got {tuple(q_shape)}")
+    q_shape, shape, table = q.shape, k_cache.shape, block_table.shape
+    if not (len(q_shape) == 3 and len(shape) == 4 and len(table) == 2):
+        _refuse_attn_paged(q, k_cache, v_cache, block_table, lengths, o, lse)
     n, heads, dim = q_shape
-    shape, code, ks, vs = _pages(k_cache, v_cache)
     pages, kv_heads, page, cache_dim = shape
-    if cache_dim != dim:
-        raise ValueError(f"q has head dimension {dim}, the cache {cache_dim}")
-    dtype = k_cache.dtype
-    q_code = _TYPE_CODES.get(q.dtype)
-    if q_code != 2 and q_code != code:
-        raise TypeError(f"q must be float32 or of the cache's type {dtype}, got {q.dtype}")
-    qs = q.stride()
-    if qs[2] != 1:
-        raise ValueError("the head dimension of q must be contiguous")
-    blocks, row = _block_table(block_table, n)
-    if lengths.dtype is not torch.int32 or lengths.shape != (n,) or not lengths.is_contiguous():
-        _vector(lengths, n, torch.int32, "lengths")
+    rows, blocks = table
+    dtype, q_dtype = k_cache.dtype, q.dtype
     if o is None:
         o = _new(q, (n, heads, dim), dtype, stream)
-    elif o.shape != q_shape:
-        raise ValueError(f"o must have q's shape {(n, heads, dim)}, got {tuple(o.shape)}")
-    elif o.dtype is not dtype:
-        raise TypeError(f"o must be of the cache's type {dtype}, got {o.dtype}")
-    elif not o.is_contiguous():
-        raise ValueError("o must be contiguous")
-    if lse is not None:
-        if lse.shape != (n, heads) or not lse.is_contiguous():
-            raise ValueError(f"lse must be a contiguous ({n}, {heads}), got {tuple(lse.shape)}")
-        if lse.dtype is not torch.float32:
-            raise TypeError(f"lse must be torch.float32, got {lse.dtype}")
+    qs, ks, vs, ts = q.stride(), k_cache.stride(), v_cache.stride(), block_table.stride()
     device = q.get_device()
-    if device < 0 or not (device == k_cache.get_device() == v_cache.get_device() == block_table.get_device()
-                          == lengths.get_device() == o.get_device()) or (lse is not None and lse.get_device() != device):
-        _on_gpu(q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, o=o,
-                **({} if lse is None else {"lse": lse}))
+    # (looked at together, and one by one only to say what is wrong)
+    if not (v_cache.shape == shape and cache_dim == dim and rows == n and lengths.shape == (n,) and o.shape == q_shape
+            and v_cache.dtype is dtype and (q_dtype is dtype or q_dtype is torch.float32) and o.dtype is dtype
+            and lengths.dtype is torch.int32 and block_table.dtype is torch.int32 and dtype in _CACHE_TYPES
+            and qs[2] == 1 and ks[3] == 1 and vs[3] == 1 and (ts[1] == 1 or blocks <= 1) and lengths.is_contiguous()
+            and o.is_contiguous() and device == k_cache.get_device() == v_cache.get_device() == block_table.get_device()
+            == lengths.get_device() == o.get_device() >= 0):
+        _refuse_attn_paged(q, k_cache, v_cache, block_table, lengths, o, lse)
+    lse_ptr = 0
+    if lse is not None:
+        if not (lse.shape == (n, heads) and lse.dtype is torch.float32 and lse.is_contiguous() and lse.get_device() == device):
+            _refuse_attn_paged(q, k_cache, v_cache, block_table, lengths, o, lse)
+        lse_ptr = lse.data_ptr()
     launch_stream = _stream_of(stream, device)
     if workspace is None:
         workspace = _own_workspace(q, device, stream, (device, heads, kv_heads, dim))
@@ -765,9 +787,9 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
         if workspace.get_device() != device:
             _on_gpu(q=q, workspace=workspace)
     packed = _PAGED_ATTN_ARGS.pack(
-        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], code, pages, kv_heads, page, dim, 0,
-        q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        workspace.data_ptr(), workspace.nbytes, qs[0], qs[1], row, n, heads, blocks, q_code,
+        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], _TYPE_CODES[dtype], pages, kv_heads,
+        page, dim, 0, q.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), o.data_ptr(), lse_ptr, workspace.data_ptr(),
+        workspace.nbytes, qs[0], qs[1], ts[0], n, heads, blocks, _TYPE_CODES[q_dtype],
         1.0 / dim ** 0.5 if scale is None else scale, 0)
     _call((_lib or lib()).spork_attn_sm100_paged, packed, device, launch_stream, "spork_attn_sm100_paged")
     return o
