@@ -374,9 +374,9 @@ typedef struct spork_paged_cache {
  * from free_pages, in the order of the requests, from entry *free_used on, and
  * entered into its row of block_table (in place; other entries stay as they are).
  * A request is refused, i.e. left as it was with no slots for its tokens, if a length
- * is negative, its table row (or 2^31 - 1 tokens) or the slot map is too short, or the free pages left
- * by the requests before it (refused for want of pages or not) do not cover its own;
- * one that needs no page is not refused for want of pages.  Written:
+ * is negative, its table row (or 2^31 - 1 tokens) or the slot map is too short, or
+ * the free pages left by the requests before it (refused for want of pages or not) do
+ * not cover its own; one that needs no page is not refused for want of pages.  Written:
  *   slots[max_tokens]      the new tokens' slots, request by request; -1 where there
  *                          is none (a refused request, behind the last token, a
  *                          negative page)
@@ -433,7 +433,8 @@ int spork_paged_sm100_store(const spork_paged_store_args* args, void* stream);
  * read.  Entries of a table row behind the last page that is needed, and rows of that
  * page behind the last key, may hold anything.  head_dim 64 or 128; page_size 8, 16,
  * 32 or a multiple of 64; heads a multiple of kv_heads; k, v and their strides
- * multiples of 16 bytes; scale positive and finite.
+ * multiples of 16 bytes; scale positive and finite; requests * kv_heads * keys that a
+ * table row has room for below about 2^37 (SPORK_ERR_TOO_LARGE).
  * A value of V that is not finite makes what it counts in so too (NaN, where the
  * definition may give an infinity); fp32 q has to lie within the cache type's range.
  * `workspace`: device memory of spork_attn_sm100_paged_workspace bytes, 16-byte

@@ -749,10 +749,11 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     and ``v_cache`` are (num_pages, kv_heads, page_size, head_dim), the first three dimensions in any order in memory;
     ``block_table`` (R, max_blocks) and ``lengths`` (R,) are int32.  ``o`` (contiguous) has the cache's type.  ``lse``, if
     given, is (R, heads) float32 and receives the logarithm of each softmax's sum.  A request of length 0 gets zeros (lse
-    -inf); one with a length outside its table row or a page outside the cache gets NaN.  ``workspace`` is a contiguous
-    CUDA tensor of attn_paged_workspace bytes, zero when it is first used and left so by every call; launches that may run at
-    the same time (other streams, other captured graphs) need one each.  Without one, a stream's launches share one that is
-    kept for the stream, and a captured launch gets its own."""
+    -inf); one with a length outside its table row or a page outside the cache gets NaN.  No gradient goes through it.
+
+    ``workspace`` is a contiguous CUDA tensor of attn_paged_workspace bytes, zero when it is first used and left so by every
+    call; launches that may run at the same time (other streams, other captured graphs) need one each.  Without one, a
+    stream's launches share one that is kept for the stream, and a captured launch gets its own."""
     torch = _T or _bind_torch()
     q_shape, shape, table = q.shape, k_cache.shape, block_table.shape
     if not (len(q_shape) == 3 and len(shape) == 4 and len(table) == 2):

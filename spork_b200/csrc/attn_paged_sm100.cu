@@ -7,7 +7,7 @@
 // equal run of that list, whatever the lengths (they are known on the device only).  A block joins what it computes of
 // one (request, key head) and writes the result if it has all of it.  Otherwise it leaves a partial result (running
 // maximum, sum, unnormalised output) in the workspace and counts itself in; the block that comes last joins the parts,
-// eight at a time, in the order of the keys.  So one launch does, and what is added to what does not depend on who was last.
+// in the order of the keys.  So one launch does, and what is added to what does not depend on who was last.
 //
 // One warp copies the pages with TMA: the cache is a 5-dimensional tensor (64 elements, page rows, halves of the head
 // dimension, heads, pages) with the strides that it has, so any order in memory is one tensor map; a box is a page's
@@ -22,7 +22,14 @@
 // feed.)  With 9 or more query heads to a key head the warps form 2 or 4 groups that share the unit, 8 heads each.
 // Each warp runs its own online softmax.  Its maximum follows the scores lazily: only when one has grown by more than
 // 2^8 over it are the row's lanes asked and the sums rescaled, so most units need no exchange between lanes at all.  The
-// warps of a group are joined once per (request, key head), pairwise: a warp that has handed its sums over goes on.
+// warps of a group are joined once per (request, key head): each gets the others' sums for its share of the columns, and
+// writes that (or leaves it in the workspace, and joins that share of the parts).
+//
+// Measured (us a launch, in a stream of them; the share of the measured copy rate): 64 requests of 4096..8192 keys, 64 query
+// and 8 key heads of 128, bf16, 1.68 GB: 246 (104 %); 16 of 4096 keys, 16 heads of 128, 537 MB: 85 (96 %); one of 131072
+// keys, 32 / 8 heads: 86 (95 %); 23 of 1..6001 keys, 40 / 8 heads, fp32 q: 47 (82 %).  Of a short launch's time about 1.5 us
+// pass until a block knows its run (one trip to memory and a scan), 2 until its first keys are there, and 1.5 to 2.5 in the
+// joining of parts.  ncu: local memory 0, tensor pipe about 10 % busy, stalls almost all on loads.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -57,12 +64,19 @@ constexpr int kBlocksPerSm = 2;
 constexpr int kComputeRegs = 192, kCopyRegs = 64;
 // setmaxnreg.inc waits, without a limit, for registers to be free: the trade must fit what the block was launched with
 static_assert(kComputeRegs + kCopyRegs <= 2 * (65536 / (kThreads * kBlocksPerSm)), "register trade exceeds the launch allocation");
-constexpr int kPairCost = 1;       // what a (request, key head) costs a block besides its units, in units
-constexpr int kWhole = 4;          // a (request, key head) of so many units or fewer is not cut
-constexpr int kMinRun = 2;         // places of a block's run, at least
+// What a (request, key head) costs a block besides its units, in units: its end takes about as long as a unit's work.
+constexpr int kPairCost = 1;
+// A (request, key head) of so many units or fewer is not cut: joining parts takes longer than three units do (one request of
+// 317 keys, units of 128: 6.5 us whole, 7.5 in three parts).
+constexpr int kWhole = 4;
+// Places of a block's run, at least: of 4, short requests queue up behind one another (4 requests of 128 keys, 8 key heads:
+// 6.6 us with 2, 9.4 with 4); of 1, long ones come to more parts (no slower where measured, but never faster).
+constexpr int kMinRun = 2;
 constexpr int kMaxRows = 64;       // rows of a TMA box
 constexpr int kLengths = 512;      // requests whose lengths a block keeps in shared memory
-constexpr int kFan = 10;           // parts that are joined at a time
+// Parts that are joined at a time.  One request of 8192 keys on all SMs, 37 parts: 13.3 us with 10, 13.5 with 16, 14.4 with 40
+// in one step.
+constexpr int kFan = 10;
 constexpr int kLevels = 3;         // of joining: kFan^kLevels is more than the blocks of a launch
 
 // kGroups groups of warps share a unit, each with 8 query heads of its own.
@@ -531,12 +545,11 @@ __device__ __forceinline__ uint32_t place_of(int first, int first_slot, int i)
 
 // A warp counts its share of this block's part in, which it has written.  The last of every kFan joins these in order and
 // leaves the result where the first of them was, and so on; the last of all writes the row of the output (o null: there is
-// none). 
-// (Few parts are under way at a time: the main loop's registers are all in use, and it bears no spills.  With 200 bytes of
-// them to a thread the kernel took up to 1.4 times as long: beside the stages little of L1 is left to keep them.)
+// none).  (The main loop bears no spills for this: with 200 bytes of them to a thread the kernel took up to 1.4 times as
+// long, since little of L1 is left beside the stages.)
 template <typename T, int kShare>
-__device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, float* part_o, int first, int parts, int first_slot,
-                                        T* o, float* lse)
+__device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, float* part_o, int first, int parts,
+                                           int first_slot, T* o, float* lse)
 {
     const int lane = threadIdx.x % 32;
     int mine = (int)blockIdx.x - first, step = 1;  // part i of a level is where part i * step of the lowest one was

@@ -243,7 +243,7 @@ __device__ __forceinline__ void load_elements(const T* p, T (&x)[8])
     uint4* to = reinterpret_cast<uint4*>(x);
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-        to[i] = __ldg(from + i);
+        to[i] = from[i];  // (no read-only load: the kernel before this one may still have been writing when this one began)
     }
 }
 
