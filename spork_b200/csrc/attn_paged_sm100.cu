@@ -26,10 +26,11 @@
 // writes that (or leaves it in the workspace, and joins that share of the parts).
 //
 // Measured (us a launch, in a stream of them; the share of the measured copy rate): 64 requests of 4096..8192 keys, 64 query
-// and 8 key heads of 128, bf16, 1.68 GB: 246 (104 %); 16 of 4096 keys, 16 heads of 128, 537 MB: 85 (96 %); one of 131072
+// and 8 key heads of 128, bf16, 1.68 GB: 246..248 (104 %); 16 of 4096 keys, 16 heads of 128, 537 MB: 85..87 (94..96 %); one of 131072
 // keys, 32 / 8 heads: 86 (95 %); 23 of 1..6001 keys, 40 / 8 heads, fp32 q: 47 (82 %).  Of a short launch's time about 1.5 us
 // pass until a block knows its run (one trip to memory and a scan), 2 until its first keys are there, and 1.5 to 2.5 in the
-// joining of parts.  ncu: local memory 0, tensor pipe about 10 % busy, stalls almost all on loads.
+// joining of parts.  ncu (16 requests of the first shape): no local memory, mma.sync
+// at 17 % of its peak rate; of 11.5 warps between two instructions 5.9 wait for memory and 2.5 for a fixed latency.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1017,7 +1018,9 @@ static EncodeTiledFn encode_tiled_fn()
     return fn;
 }
 
-// Query heads of a key head are taken 8, 16 or 32 at a time (groups of warps that share the keys in shared memory).
+// Query heads of a key head are taken 8, 16 or 32 at a time (groups of warps that share the keys in shared memory): the
+// fewest that hold them all, as empty rows cost a group's time.  us with 8 / 16 / 32 for 64 requests of 4096..8192 keys, 8 to
+// one, D = 128: 248 / 255 / 331; the same with 16 to one, with 16 / 32: 248 / 346.
 static int groups_of(int group) { return group <= kHeads ? 1 : group <= 2 * kHeads ? 2 : 4; }
 static int blocks_of(int sm_count) { return kBlocksPerSm * sm_count; }
 
