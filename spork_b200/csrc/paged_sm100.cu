@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(kTableThreads) tables_kernel(const spork_paged
         a.info[2] = refused;
         a.info[3] = (int32_t)pages;
     }
-    for (int i = at; i < granted; i += stride) {
+    for (uint32_t j = at; j < (uint32_t)granted; j += stride) {  // (unsigned: one step past 2^31 - 1 pages is still a number)
+        const int i = (int)j;
         const int r = last_at_most(first_page, n, i);
         const uint32_t old = page_of.for_tokens(held_of[r]);
         a.block_table[r * a.table_stride + old + (i - first_page[r])] = a.free_pages[used + i];

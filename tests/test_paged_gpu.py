@@ -83,6 +83,30 @@ def test_tables_far_numbers_and_odd_lists(sp, cuda):
     _run_tables(sp, cuda, [0, 0], [0, 0], [[], []], [], 0, 16, 2)
 
 
+def test_tables_of_nearly_2_31_pages(sp, cuda):
+    # pages of one token, nearly all that a step can grant: page numbers near the end of 31 bits, 34 GB of lists
+    import torch
+
+    requests, each = 16384, 131071
+    pages = requests * each
+    assert I32 - 148 * 1024 < pages < I32
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    lengths = torch.zeros(requests, dtype=torch.int32, device=cuda)
+    new = torch.full((requests,), each, dtype=torch.int32, device=cuda)
+    table = torch.full((requests, each), -7, dtype=torch.int32, device=cuda)
+    free = torch.arange(pages, dtype=torch.int32, device=cuda)
+    used = torch.zeros(1, dtype=torch.int32, device=cuda)
+    slots, offsets, after, info = sp.paged_tables(lengths, new, table, free, used, page_size=1, max_tokens=pages)
+    assert info.tolist() == [pages, pages, 0, pages]
+    assert torch.equal(after, new) and offsets[-1].item() == pages
+    assert torch.equal(table.view(-1), free)
+    for at in range(0, pages, 1 << 28):
+        assert torch.equal(slots[at:at + (1 << 28)], free[at:at + (1 << 28)].to(torch.int64)), at
+    del table, free, slots
+    torch.cuda.empty_cache()
+
+
 def test_tables_of_no_requests(sp, cuda):
     import torch
 
