@@ -48,7 +48,8 @@ def _run_tables(sp, cuda, held, new, table, free, used, page, max_tokens, stride
 
 @pytest.mark.parametrize("requests,page,most_held,most_new,room", [
     (1, 16, 0, 1, 0), (1, 1, 5, 9, 4), (256, 16, 4000, 1, 0), (33, 48, 500, 700, 11), (1000, 32, 300, 40, 100), (2, 7, 100, 50000, 1),
-    (4097, 64, 200, 3, 0), (16384, 16, 90, 2, 5), (1025, 128, 0, 300, 1000)])
+    (4097, 64, 200, 3, 0), (16384, 16, 90, 2, 5), (1025, 128, 0, 300, 1000),
+    (700, 48, 500, 600, 3), (5000, 7, 30, 90, 1)])  # these two: four tokens to a thread, requests and pages that end inside
 def test_tables_match_the_rules(sp, cuda, requests, page, most_held, most_new, room):
     rng = random.Random(requests * 1000 + page)
     held = [rng.randint(0, most_held) for _ in range(requests)]
@@ -81,6 +82,21 @@ def test_tables_far_numbers_and_odd_lists(sp, cuda):
     _run_tables(sp, cuda, [0], [3], [[-7]], [I32], 0, I32, 3)
     _run_tables(sp, cuda, [I32 - 1, I32 - 1, I32], [1, 2, 0], [[4, -7]] * 3, [I32, 8], 0, I32, 3)
     _run_tables(sp, cuda, [0, 0], [0, 0], [[], []], [], 0, 16, 2)
+
+
+def test_tables_write_slots_wherever_they_begin(sp, cuda):
+    # a slot map on no boundary of 16 bytes, large enough for four tokens to a thread; nothing around it is touched
+    import torch
+
+    i32 = dict(dtype=torch.int32, device=cuda)
+    tokens = 160001
+    around = torch.full((tokens + 2,), -9, dtype=torch.int64, device=cuda)
+    slots, _, _, info = sp.paged_tables(torch.tensor([5], **i32), torch.tensor([tokens - 1], **i32),
+                                        torch.zeros((1, 10001), **i32), torch.arange(1, 10001, **i32),
+                                        torch.tensor([0], **i32), page_size=16, slots=around[1:-1])
+    assert info.tolist() == [10000, tokens - 1, 0, 10000]
+    assert torch.equal(slots[:-1], torch.arange(5, tokens + 4, device=cuda)) and slots[-1] == -1
+    assert around[0] == -9 and around[-1] == -9
 
 
 def test_tables_of_nearly_2_31_pages(sp, cuda):
@@ -135,7 +151,9 @@ def _empty_cache(cuda, pages, kv_heads, page, dim, dtype, order, fill):
 @pytest.mark.parametrize("src,dst", [("float32", "float16"), ("float32", "bfloat16"), ("float16", "float16"), ("bfloat16", "bfloat16")])
 @pytest.mark.parametrize("tokens,kv_heads,page,dim,order,shift", [
     (1, 1, 16, 64, "heads", 0), (37, 8, 16, 128, "tokens", 0), (300, 3, 24, 64, "both", 4), (65, 5, 7, 96, "heads", 8),
-    (129, 2, 32, 128, "wide", 1), (50, 4, 1, 40, "tokens", 3), (9, 1, 64, 1, "heads", 0), (2050, 2, 64, 128, "heads", 0)])
+    (129, 2, 32, 128, "wide", 1), (50, 4, 1, 40, "tokens", 3), (9, 1, 64, 1, "heads", 0), (2050, 2, 64, 128, "heads", 0),
+    # enough blocks for four tokens to a thread: side by side in a block or not, in pieces or single elements, odd ends
+    (2401, 8, 16, 128, "tokens", 0), (7203, 2, 32, 128, "both", 4), (7150, 2, 16, 128, "heads", 0), (1777, 3, 24, 64, "wide", 1)])
 def test_store_puts_each_token_into_its_slot(sp, cuda, src, dst, tokens, kv_heads, page, dim, order, shift):
     import torch
 
