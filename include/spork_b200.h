@@ -436,7 +436,12 @@ int spork_paged_sm100_store(const spork_paged_store_args* args, void* stream);
  * multiples of 16 bytes; scale positive and finite; requests * kv_heads * keys that a
  * table row has room for below about 2^37 (SPORK_ERR_TOO_LARGE).
  * A value of V that is not finite makes what it counts in so too (NaN, where the
- * definition may give an infinity); fp32 q has to lie within the cache type's range.
+ * definition may give an infinity).
+ * Precision: products and sums are taken in 32 bits, of keys and values as they are, and of softmax weights and
+ * fp32 q as two parts of the cache's type each, which together keep 22 bits of each number with fp16 and 16 with
+ * bf16.  (fp16: weights to 2^-31 of the largest at least; elements of an fp32 q to 2^-39 of the largest of their
+ * row at least, whatever its size.)  o is rounded to the cache's type once.  scale times the largest element of a
+ * row of q has to lie within fp32's range.
  * `workspace`: device memory of spork_attn_sm100_paged_workspace bytes, 16-byte
  * aligned.  Its first SPORK_ATTN_PAGED_COUNTERS bytes must be zero before the first
  * call that uses it, and every call leaves them so (unless it was given up half way:

@@ -750,6 +750,8 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     ``block_table`` (R, max_blocks) and ``lengths`` (R,) are int32.  ``o`` (contiguous) has the cache's type.  ``lse``, if
     given, is (R, heads) float32 and receives the logarithm of each softmax's sum.  A request of length 0 gets zeros (lse
     -inf); one with a length outside its table row or a page outside the cache gets NaN.  No gradient goes through it.
+    Softmax weights, and ``q`` where it is float32, are taken as two parts of the cache's type each: 22 bits with float16, 16
+    with bfloat16, for queries of any size (beside spork_attn_sm100_paged in include/spork_b200.h).
 
     ``workspace`` is a contiguous CUDA tensor of attn_paged_workspace bytes, zero when it is first used and left so by every
     call; launches that may run at the same time (other streams, other captured graphs) need one each.  Without one, a

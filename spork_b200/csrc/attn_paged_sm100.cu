@@ -17,7 +17,8 @@
 // Four warps compute, each on keys of its own, with mma.m16n8k16.  Up to 8 query heads are rows 0-7 of the 16-row
 // operand, and rows 8-15 hold what rounding to 16 bits left over: of q, if it is fp32, and of the softmax weights.  So
 // both products are taken with about 22 (fp16) or 16 (bf16) bits of q and of the weights at no cost: the rows would have
-// been empty, and the weights' rounding, the largest error of the usual scheme, is gone.  (tcgen05 would want 64 or 128
+// been empty, and the weights' rounding, the largest error of the usual scheme, is gone.  (Rows of fp32 queries are brought
+// into the 16-bit type's range by a power of two first.)  (tcgen05 would want 64 or 128
 // rows and a trip through tensor memory for every unit; the warp instruction's rate is several times what the loads can
 // feed.)  With 9 or more query heads to a key head the warps form 2 or 4 groups that share the unit, 8 heads each.
 // Each warp runs its own online softmax.  Its maximum follows the scores lazily: only when one has grown by more than
@@ -270,6 +271,7 @@ struct Softmax {
     uint32_t q_hi[kSteps][2], q_lo[kLowQ ? kSteps : 1][2];
     float acc[D / 8][4];
     float m, l;  // of row g; l: this lane's columns only
+    float row_scale;  // kLowQ: what turns a score of row g into a power of two's exponent
     uint32_t weights[kPairs][4];
 
     // The queries as they are (kLowQ: 32 bits), on their way into the registers that begin() makes operands of.  Nothing is
@@ -302,14 +304,37 @@ struct Softmax {
         }
     }
 
-    __device__ __forceinline__ void begin()
+    // (kLowQ) Each row is brought by a power of two, which its scale takes back, to where two 16-bit parts hold it: the
+    // exponent of its largest finite element becomes 14 in fp16, so that elements down to 2^-17 of that one keep 22 bits and
+    // no smaller one is off by more than 2^-39 of it; bf16 has fp32's range, and only rows near its ends are moved.  (Sums
+    // of products with keys of any size stay within fp32 then, too.)
+    __device__ __forceinline__ void begin(float scale)
     {
         if constexpr (kLowQ) {
+            constexpr int kLeast = kBf16 ? -60 : 14, kMost = kBf16 ? 60 : 14;
+            uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    split<T>(__uint_as_float(q_hi[i][j]), __uint_as_float(q_lo[i][j]), q_hi[i][j], q_lo[i][j]);
+                    const uint32_t x = q_hi[i][j] & 0x7FFFFFFFu, y = q_lo[i][j] & 0x7FFFFFFFu;
+                    most = max(most, x < 0x7F800000u ? x : 0u);
+                    most = max(most, y < 0x7F800000u ? y : 0u);
+                }
+            }
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+            const int exponent = max((int)(most >> 23), 1) - 127;
+            // -113 .. 140: in two factors within range
+            const int up = most > 0 ? max(kLeast, min(kMost, exponent)) - exponent : 0;
+            const int up0 = up / 2, up1 = up - up0;
+            const float by0 = __int_as_float((127 + up0) << 23), by1 = __int_as_float((127 + up1) << 23);
+            row_scale = scale * __int_as_float((127 - up0) << 23) * __int_as_float((127 - up1) << 23);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    split<T>(__uint_as_float(q_hi[i][j]) * by0 * by1, __uint_as_float(q_lo[i][j]) * by0 * by1, q_hi[i][j], q_lo[i][j]);
                 }
             }
         }
@@ -328,8 +353,9 @@ struct Softmax {
     // Weights of a unit's keys, whose rows for ldmatrix are at `row`; `keys` of them count (kRagged: not all, and the rest
     // may be anything).
     template <bool kRagged>
-    __device__ __forceinline__ void take_keys(const uint32_t (&row)[kPairs], uint32_t base, uint32_t half, int keys, float scale)
+    __device__ __forceinline__ void take_keys(const uint32_t (&row)[kPairs], uint32_t base, uint32_t half, int keys, float scale_log2e)
     {
+        const float scale = kLowQ ? row_scale : scale_log2e;
         const int lane = threadIdx.x % 32, t = lane % 4, matrix = lane / 8, row8 = lane % 8;
         float s[2 * kPairs][4];
 #pragma unroll
@@ -863,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
                 break;
             }
             if (which.x == 0) {
-                sm.begin();
+                sm.begin(p.scale_log2e);
                 bad = 0;
             }
             bad |= flags & kBad;

@@ -77,3 +77,25 @@ def tolerances(dtype, keys, dim, ref, weighted, size, fp32_q):
     tol_o = half * ref.abs() + (1 + half) * inner[:, None] * weighted + torch.finfo(dtype).smallest_normal * half
     tol_lse = e + (keys + 64) * 2.0 ** -23 + 2.0 ** -23 * (size + math.log(max(keys, 1)) + 1)
     return tol_o, tol_lse
+
+
+def tolerances_of_fp32_queries(dtype, q, k, scale, ref, weighted, size):
+    """The same for fp32 queries of any size, over the keys k (kv_heads, keys, D) of one request.
+
+    A query's row is brought by a power of two, which is exact, to where the cache type has room below it, and taken as two
+    parts of that type.  What the two leave over: the second part is off by eps / 2 of what the first one left, which is
+    eps / 2 of the element, so (eps / 2)^2 of the element; and by half of the type's smallest step.  That step is fp16's
+    2^-24, and the row's largest element is brought to 2^14 at least: 2^-39 of that one.  (bf16: 2^-134 beside 2^-60 at
+    least, nothing; an fp32 subnormal has no more bits than the two parts.)  The rest is as above."""
+    import torch
+
+    heads, dim = q.shape
+    kv_heads, keys, _ = k.shape
+    half = torch.finfo(dtype).eps / 2
+    sums = k.double().abs().sum(2).amax(1).repeat_interleave(heads // kv_heads)  # per head, of the key with the largest one
+    least = 2.0 ** -39 if dtype == torch.float16 else 2.0 ** -74
+    e = size * ((dim + 8) * 2.0 ** -23 + half * half) + least * q.double().abs().amax(1) * sums * scale + 2.0 ** -21
+    inner = 2 * e + half * half + keys * 2.0 ** -31 + (keys + 64) * 2.0 ** -23
+    tol_o = half * ref.abs() + (1 + half) * inner[:, None] * weighted + torch.finfo(dtype).smallest_normal * half
+    tol_lse = e + (keys + 64) * 2.0 ** -23 + 2.0 ** -23 * (size + math.log(max(keys, 1)) + 1)
+    return tol_o, tol_lse

@@ -351,6 +351,61 @@ def test_attention_large_scores_and_small_weights(sp, cuda):
         case.check(*case.run(sp))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (9, 1, 128), (40, 2, 128), (16, 16, 64)])
+@pytest.mark.parametrize("dtype,size", [("float16", s) for s in (1e-3, 1e-4, 1e-5, 1e-6, 1e-9, 1e-30, 1e-38, 1e6, 1e30)]
+                         + [("bfloat16", s) for s in (1e-6, 1e-30, 1e-36, 1e-38, 1e30, 3e37)])
+def test_attention_of_fp32_queries_of_any_size(sp, cuda, dtype, size, heads, kv_heads, dim):
+    """Queries far below or above the cache type's range, with a scale that makes scores of a size around one of them: rows
+    keep their bits, each by itself (they differ by up to 2^20 here, one is zero), and so does lse."""
+    import torch
+
+    dtype = getattr(torch, dtype)
+    case = Paged(cuda, [700, 1, 63, 0, 129], heads, kv_heads, dim, 16, dtype, torch.float32, seed=heads)
+    row = torch.arange(len(case.lengths) * heads, device=cuda).view(-1, heads, 1) * 7 % 11
+    case.q = (case.q.clamp(-4, 4).double() * 2.0 ** (-2.0 * row) * size).float()
+    case.q[0, 3] = 0.0
+    scale = 1.0 / dim ** 0.5 / size
+    if scale > 1e38:
+        scale = 1e38
+    o, lse = case.run(sp, scale=scale)
+    scale = torch.tensor(scale, dtype=torch.float32).item()
+    for r, n in enumerate(case.lengths):
+        ref, ref_lse, weighted, sizes = paged_plain.attention(case.q[r], case.k[r], case.v[r], scale)
+        if n == 0:
+            assert (o[r] == 0).all() and (lse[r] == -math.inf).all()
+            continue
+        tol_o, tol_lse = paged_plain.tolerances_of_fp32_queries(dtype, case.q[r], case.k[r], scale, ref, weighted, sizes)
+        err, err_lse = (o[r].double() - ref).abs() / tol_o, (lse[r].double() - ref_lse).abs() / tol_lse
+        assert err.max() <= 1 and err_lse.max() <= 1, f"request {r}: o {err.max()}, lse {err_lse.max()} of what is allowed"
+
+
+def test_attention_of_fp32_queries_with_infinities(sp, cuda):
+    """An element of q that is not finite says nothing about how its row is scaled: its scores are infinite or NaN as the
+    definition has them, and the other rows are what they are without it."""
+    import torch
+
+    for dtype in (torch.float16, torch.bfloat16):
+        case = Paged(cuda, [100, 40], 4, 2, 64, 16, dtype, torch.float32, seed=8)
+        case.q = case.q * 1e-6
+        case.q[0, 1, 5], case.q[0, 2, 6] = math.inf, math.nan
+        case.k[0][0, :, 5] = -1.0 - case.k[0][0, :, 5].abs()  # row 1's scores: all but one are -infinity
+        case.k[0][0, 33, 5] = 0.0
+        for i in range(100):
+            case.kc[case.table[0, i // 16].item(), 0, i % 16] = case.k[0][0, i]
+        o, lse = case.run(sp, scale=1e5)
+        assert o[0, 1].isnan().all() and o[0, 2].isnan().all() and lse[0, 1].isnan() and lse[0, 2].isnan()  # 0 times infinity
+        case.k[0][0, 33, 5] = -2.0
+        case.kc[case.table[0, 2].item(), 0, 1] = case.k[0][0, 33]
+        o, lse = case.run(sp, scale=1e5)
+        assert o[0, 1].isnan().all() and lse[0, 1] == -math.inf  # every key is masked: nothing to divide by
+        scale = torch.tensor(1e5, dtype=torch.float32).item()
+        for r, rows in ((0, [0, 3]), (1, [0, 1, 2, 3])):
+            q = case.q[r].nan_to_num(0, 0, 0)
+            ref, _, weighted, sizes = paged_plain.attention(q, case.k[r], case.v[r], scale)
+            tol, _ = paged_plain.tolerances_of_fp32_queries(dtype, q, case.k[r], scale, ref, weighted, sizes)
+            assert ((o[r].double() - ref).abs() <= tol)[rows].all()
+
+
 def test_attention_infinities_and_nan_in_keys_that_count(sp, cuda):
     """An infinite score is NaN, as in the definition (infinity minus infinity); one of -infinity is a masked key; a NaN is a
     NaN; the other requests do not notice."""
