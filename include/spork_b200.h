@@ -408,7 +408,9 @@ int spork_paged_sm100_tables(const spork_paged_tables_args* args, void* stream);
  * cache's type if it is of another one.  src_type is the cache's type or
  * SPORK_TYPE_F32 (what the GEMMs write).  A slot outside the cache (-1, say)
  * writes nothing.  Slots within the cache must differ: of two tokens with the same
- * one, either's values may remain, piece by piece. */
+ * one, either's values may remain, piece by piece.  A token's keys and values together
+ * come to fewer than about 2^31 pieces (SPORK_ERR_TOO_LARGE): of 8 elements where
+ * pointers, head_dim and strides allow 16 bytes of the cache at a time, else of one. */
 typedef struct spork_paged_store_args {
     spork_paged_cache cache;
     const void* k;

@@ -489,6 +489,11 @@ extern "C" int spork_paged_sm100_store(const spork_paged_store_args* args, void*
         (reinterpret_cast<uintptr_t>(a.slots) % 8)) {
         return SPORK_ERR_BAD_ARGUMENT;
     }
+    // a token's pieces are counted in 32 bits, with a block's step behind the last one
+    const int64_t pieces = 2 * (int64_t)a.cache.kv_heads * (a.cache.head_dim / (spork::paged_sm100::store_aligned(a) ? 8 : 1));
+    if (pieces > 0x7FFFFFFF - spork::paged_sm100::kStoreThreads) {
+        return SPORK_ERR_TOO_LARGE;
+    }
     spork::DeviceState* dev = nullptr;
     const int rc2 = spork::current_device_state(&dev);
     if (rc2) {

@@ -61,6 +61,18 @@ def test_store_refuses(sp, change, code):
     assert sp.lib().spork_paged_sm100_store(store_args(**change), None) == code
 
 
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,shift", [
+    (1, INT_MAX, 0), (1 << 30, 1, 0), (1 << 15, 1 << 15, 1), (INT_MAX, INT_MAX, 0), (3, 715827883, 0), ((1 << 30) - 100, 1, 0),
+    (1 << 16, 1 << 17, 0)])  # the last one in pieces of 8 elements
+def test_store_refuses_rows_of_more_pieces_than_32_bits_count(sp, kv_heads, head_dim, shift):
+    # (one row to a page, so that no stride comes into it but that of the heads)
+    c = cache(kv_heads=kv_heads, head_dim=head_dim, page_size=1, num_pages=1, kh=head_dim, vh=head_dim, k=FAKE + 2 * shift)
+    assert sp.lib().spork_paged_sm100_store(store_args(c, kh=head_dim, vh=head_dim, tokens=1), None) == 10006
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(requests=-1), 10002), (dict(heads=3), 10002), (dict(heads=-2), 10002), (dict(max_blocks=-1), 10002),
     (dict(table_stride=7), 10002), (dict(q=0), 10001), (dict(q=FAKE + 1), 10001), (dict(q_type=1), 10001),
