@@ -68,6 +68,10 @@ inline int check_cache(const spork_paged_cache& c)
             if (step < covered || step > (int64_t)1 << 40) {
                 return SPORK_ERR_BAD_ARGUMENT;
             }
+            // places are counted in 64 bits, and no address space holds 2^57 bytes
+            if (n - 1 > (((int64_t)1 << 56) - covered) / step) {
+                return SPORK_ERR_TOO_LARGE;
+            }
             covered += (n - 1) * step;
         }
     }

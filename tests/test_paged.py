@@ -73,6 +73,18 @@ def test_store_refuses_rows_of_more_pieces_than_32_bits_count(sp, kv_heads, head
     assert sp.lib().spork_paged_sm100_store(store_args(c, kh=head_dim, vh=head_dim, tokens=1), None) == 10006
 
 
+@pytest.mark.parametrize("halves", ["k", "v", "kv"])
+@pytest.mark.parametrize("change", [
+    # rows that cover 2^71 elements, which 64 bits would wrap to less than nothing, and pages that lie inside them
+    dict(page_size=INT_MAX - 63, r=1 << 40, p=1 << 40, num_pages=INT_MAX), dict(page_size=1 << 30, r=1 << 40, p=1 << 40),
+    dict(page_size=1 << 20, r=1 << 40), dict(num_pages=INT_MAX, p=1 << 40), dict(num_pages=1 << 24, p=1 << 40, h=1 << 40)])
+def test_a_cache_that_covers_more_than_an_address_space_is_refused(sp, change, halves):
+    sizes = {k: v for k, v in change.items() if len(k) > 1}
+    c = cache(**sizes, **{half + k: v for half in halves for k, v in change.items() if len(k) == 1})
+    assert sp.lib().spork_paged_sm100_store(store_args(c), None) in (10001, 10006)
+    assert sp.lib().spork_attn_sm100_paged(attn_args(c), None) in (10001, 10006)
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(requests=-1), 10002), (dict(heads=3), 10002), (dict(heads=-2), 10002), (dict(max_blocks=-1), 10002),
     (dict(table_stride=7), 10002), (dict(q=0), 10001), (dict(q=FAKE + 1), 10001), (dict(q_type=1), 10001),
