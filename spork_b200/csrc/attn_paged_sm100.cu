@@ -1081,9 +1081,9 @@ static int fill_shape(Params& p, int requests, int heads, int kv_heads, int head
     p.head_units = (group + unit_heads - 1) / unit_heads;
     const int64_t capacity = (int64_t)max_blocks * page_size;
     p.capacity = capacity < 0x7FFFFFFF ? (int32_t)capacity : 0x7FFFFFFF;
-    // places in the list, at most
-    const int64_t places = (p.capacity / (8192 / head_dim) + 1 + kPairCost) * (int64_t)requests * kv_heads * p.head_units;
-    return places < 0x7FFFFFFF ? 0 : SPORK_ERR_TOO_LARGE;
+    // places in the list, at most: of one request (below 2^57), and of all of them
+    const int64_t places = (p.capacity / (8192 / head_dim) + 1 + kPairCost) * (int64_t)kv_heads * p.head_units;
+    return requests == 0 || places <= 0x7FFFFFFE / requests ? 0 : SPORK_ERR_TOO_LARGE;
 }
 
 struct Workspace {

@@ -237,3 +237,11 @@ def test_plan_refuses(sp):
     # more places in the list than 32 bits number: 2^25 units a request
     with pytest.raises(ValueError):
         sp.attn_paged_plan([100] * 100, 0, heads=8, kv_heads=2, head_dim=128, page_size=64, max_blocks=1 << 25)
+
+
+@pytest.mark.parametrize("requests,kv_heads,dim,blocks", [(4096, 1 << 30, 128, (1 << 25) - 2), (4096, INT_MAX, 128, 1 << 20),
+                                                          (32768, 1 << 24, 128, (1 << 25) - 2), (8192, INT_MAX, 64, 1 << 20)])
+def test_plan_refuses_more_places_than_64_bits_number(sp, requests, kv_heads, dim, blocks):
+    # the product wraps 64 bits, to zero or less (lengths of zero, so that nothing is walked through where it is not refused)
+    with pytest.raises(ValueError):
+        sp.attn_paged_plan([0] * requests, 0, heads=kv_heads, kv_heads=kv_heads, head_dim=dim, page_size=64, max_blocks=blocks)
