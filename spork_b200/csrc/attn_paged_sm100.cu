@@ -1012,10 +1012,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             if (units_of<Cfg::kTile>(p, len) == 0) {
                 const uint32_t fill = len == 0 ? 0u : pack<T>(NAN, NAN);
                 uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + (int64_t)r * p.heads * D);
-                for (int i = threadIdx.x; i < p.heads * (D / 2); i += kComputeWarps * 32) {
+                for (int64_t i = threadIdx.x; i < (int64_t)p.heads * (D / 2); i += kComputeWarps * 32) {
                     o[i] = fill;
                 }
-                for (int i = threadIdx.x; p.lse && i < p.heads; i += kComputeWarps * 32) {
+                for (int64_t i = threadIdx.x; p.lse && i < p.heads; i += kComputeWarps * 32) {
                     p.lse[(int64_t)r * p.heads + i] = len == 0 ? -INFINITY : NAN;
                 }
             }

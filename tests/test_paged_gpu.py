@@ -471,6 +471,25 @@ def test_attention_without_pages_or_columns(sp, cuda):
     assert sp.attn_paged(q[:0], c, c, table[:0], lens[:0]).shape == (0, 4, 64)
 
 
+def test_attention_of_an_empty_request_with_2_31_words_of_output(sp, cuda):
+    # (queries that are one row, and a cache without pages: only the output takes memory, 8.6 GB)
+    import torch
+
+    heads, dim = 1 << 26, 64
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB")
+    q = torch.ones((1, 1, dim), dtype=torch.float16, device=cuda).expand(1, heads, dim)
+    c = torch.empty((0, heads // 32, 8, dim), dtype=torch.float16, device=cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    o = torch.full((1, heads, dim), 9.0, dtype=torch.float16, device=cuda)
+    lse = torch.full((1, heads), 9.0, device=cuda)
+    sp.attn_paged(q, c, c, torch.zeros((1, 0), **i32), torch.zeros(1, **i32), o, lse=lse)
+    sp.status()
+    assert not o.any() and (lse == -math.inf).all()
+    del o, lse
+    torch.cuda.empty_cache()
+
+
 def test_attention_writes_its_outputs_and_nothing_else(sp, cuda):
     import torch
 
