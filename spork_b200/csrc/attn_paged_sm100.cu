@@ -825,14 +825,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             plan = next;
             next = look_ahead();
         }
-        if (!ok) {
-            // copies that are still under way end before the block does (each wait has its limit)
-            for (uint32_t s = 0; s < Cfg::kStages; ++s) {
-                const uint32_t fills = used / Cfg::kStages + (s < used % Cfg::kStages ? 1 : 0);
-                if (fills > 0) {
-                    volatile uint32_t not_aborted = 0;
-                    mbar_wait(smem_u32(&bars.full[s]), (fills - 1) & 1u, &not_aborted);
-                }
+        // Copies that are still under way end before the block does, also where only a computing warp has given up (each
+        // wait has its limit).
+        for (uint32_t s = 0; s < Cfg::kStages; ++s) {
+            const uint32_t fills = used / Cfg::kStages + (s < used % Cfg::kStages ? 1 : 0);
+            if (fills > 0) {
+                volatile uint32_t not_aborted = 0;
+                mbar_wait(smem_u32(&bars.full[s]), (fills - 1) & 1u, &not_aborted);
             }
         }
     } else {

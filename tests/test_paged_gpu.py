@@ -617,6 +617,33 @@ def test_captured_graphs_follow_the_lengths(sp, cuda):
             assert torch.equal(w, o)
 
 
+def test_after_a_wait_that_ran_out(sp, cuda):
+    """A launch that was given up may leave its workspace's counters as they were: once status() has said so, no kept
+    workspace is used again, and the next calls of every stream are right."""
+    import torch
+
+    from spork_b200 import api
+
+    case = Paged(cuda, [3000, 17, 800], 8, 2, 128, 16, torch.bfloat16, seed=12)
+    side = torch.cuda.Stream()
+    want = case.run(sp)[0]
+    side.wait_stream(torch.cuda.current_stream())
+    sp.attn_paged(case.q, case.kc, case.vc, case.table, case.len, stream=side)
+    torch.cuda.synchronize()
+    kept = list(api._workspaces.values())
+    assert len(kept) >= 2
+    for workspace in kept:
+        workspace[:65536] = 1  # as a launch would that stopped half way
+    assert sp.lib().spork_selftest_bounded_wait(1000, torch.cuda.current_stream().cuda_stream) == 0
+    with pytest.raises(sp.SporkError):
+        sp.status()
+    assert not api._workspaces
+    case.check(*case.run(sp))
+    with torch.cuda.stream(side):
+        assert torch.equal(sp.attn_paged(case.q, case.kc, case.vc, case.table, case.len), want)
+    torch.cuda.synchronize()
+
+
 def test_the_range_checked_build_agrees(sp, cuda):
     """Every kernel through libspork_b200_checked.so, in a process of its own: no range check fires, results are right."""
     import os
