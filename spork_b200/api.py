@@ -9,9 +9,11 @@ contiguous; ``c`` is (M, N) fp32.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
+import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # SPORK_B200_LIBRARY selects another build of the library (the range-checked debug build
@@ -366,7 +368,12 @@ def status(stream=None, device=None) -> None:
         detail = ctypes.c_uint32(0)
         rc = lib().spork_gemm_sm100_status(_stream_ptr(stream), ctypes.byref(detail))
     if rc != 0:
-        _workspaces.clear()  # a launch that was given up may have left its counters as they were
+        # a launch that was given up may have left its counters as they were
+        _workspaces.clear()
+        with _lent_lock:
+            for pool in _lent.values():
+                for entry in pool:
+                    entry.clean = False
         raise SporkError(rc, f"device status (detail 0x{detail.value:08x})")
 
 
@@ -476,7 +483,10 @@ _TYPE_CODES: dict = {}
 _CACHE_TYPES: set = set()
 _current_device = _raw_stream = _capturing = None
 _workspace_bytes: dict = {}  # by device and what the size depends on
-_workspaces: dict = {}       # by device and stream: the one that calls without a workspace of their own use
+_workspaces: dict = {}       # by device and stream of torch's: the one that calls without a workspace of their own use
+_lent: dict = {}             # by device: those that calls on other streams take turns with
+_lent_lock = threading.Lock()
+_LENT = 4                    # of a device, at most
 _COUNTER_BYTES = 65536       # SPORK_ATTN_PAGED_COUNTERS
 
 
@@ -531,10 +541,59 @@ def _new(like, shape, dtype, stream):
         return _T.empty(shape, dtype=dtype, device=like.device)
 
 
+class _Lent:
+    """A workspace with the event of its last use, and the handle of the stream that this was on."""
+
+    __slots__ = ("workspace", "used", "handle", "clean")
+
+
+def _whose_turn(pool: list, handle: int) -> _Lent:
+    """The pool's workspace for a launch on the stream of that handle: the one that it had last, a new one (which has no
+    memory yet), or the one that was not used for the longest time.  The pool is kept in the order of use."""
+    entry = next((e for e in pool if e.handle == handle), None)
+    if entry is not None:
+        pool.remove(entry)
+    elif len(pool) >= _LENT:
+        entry = pool.pop(0)
+    else:
+        entry = _Lent()
+        entry.workspace = entry.used = None
+        entry.clean = False
+    entry.handle = handle
+    pool.append(entry)
+    return entry
+
+
+@contextlib.contextmanager
+def _lent_workspace(like, device: int, stream):
+    """A workspace for one launch on a stream that torch did not make.  What its handle stands for may change: one of a stream
+    that was destroyed comes back, and that of the per-thread default stream means another stream in every thread.  So the
+    launches that use a workspace are put in order by an event, whatever their streams, and one is large enough for all
+    shapes and is never freed."""
+    torch = _T
+    with _lent_lock, torch.cuda.device(device):
+        if stream is None:
+            stream = torch.cuda.current_stream()
+        with torch.cuda.stream(stream):
+            entry = _whose_turn(_lent.setdefault(device, []), stream.cuda_stream)
+            if entry.workspace is None:
+                entry.used = torch.cuda.Event()
+                entry.workspace = torch.empty((attn_paged_workspace(32, 1, 128),), dtype=torch.uint8, device=like.device)
+            else:
+                stream.wait_event(entry.used)
+            if not entry.clean:
+                entry.workspace[:_COUNTER_BYTES].zero_()
+                entry.clean = True
+            try:
+                yield entry.workspace
+            finally:
+                entry.used.record(stream)
+
+
 def _own_workspace(like, device: int, stream, key):
-    """The workspace of one launch that was not given any.  Launches of one stream follow one another and share the stream's;
-    a captured launch, whose graph may be replayed beside any other, gets one of its own, with the clearing of its counters
-    in the graph."""
+    """The workspace of one launch that was not given any; None for one on a stream that torch did not make.  Launches of one
+    stream follow one another and share the stream's; a captured launch, whose graph may be replayed beside any other, gets
+    one of its own, with the clearing of its counters in the graph."""
     if stream is not None:
         with _T.cuda.stream(stream):
             return _own_workspace(like, device, None, key)
@@ -550,6 +609,8 @@ def _own_workspace(like, device: int, stream, key):
         return workspace
     at = (device, _raw_stream(device))
     workspace = _workspaces.get(at)
+    if workspace is None and at[1] and _T.cuda.current_stream(device).stream_id == at[1]:
+        return None  # (torch names its own streams otherwise than by their handles, which stay theirs)
     if workspace is None or workspace.numel() < need:
         workspace = _workspaces[at] = _T.zeros((need,), dtype=_T.uint8, device=like.device)
     return workspace
@@ -754,8 +815,10 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     with bfloat16, for queries of any size (beside spork_attn_sm100_paged in include/spork_b200.h).
 
     ``workspace`` is a contiguous CUDA tensor of attn_paged_workspace bytes, zero when it is first used and left so by every
-    call; launches that may run at the same time (other streams, other captured graphs) need one each.  Without one, a
-    stream's launches share one that is kept for the stream, and a captured launch gets its own."""
+    call (unless status() raises: zero it again then); launches that may run at the same time (other streams, other captured
+    graphs) need one each.  Without one, a stream's launches share one that is kept for the stream until the process ends (up
+    to about 10 MB), and a captured launch gets its own.  Launches on streams that torch did not make
+    (torch.cuda.ExternalStream) take turns with four workspaces a device, each waiting for the one before it."""
     torch = _T or _bind_torch()
     q_shape, shape, table = q.shape, k_cache.shape, block_table.shape
     if not (len(q_shape) == 3 and len(shape) == 4 and len(table) == 2):
@@ -784,6 +847,10 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     launch_stream = _stream_of(stream, device)
     if workspace is None:
         workspace = _own_workspace(q, device, stream, (device, heads, kv_heads, dim))
+        if workspace is None:
+            with _lent_workspace(q, device, stream) as workspace:
+                return attn_paged(q, k_cache, v_cache, block_table, lengths, o, lse=lse, scale=scale, workspace=workspace,
+                                  stream=stream)
     else:
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")

@@ -119,6 +119,22 @@ def test_supports(sp):
         assert not sp.attn_paged_supports(32, 8, 128, page)
 
 
+def test_streams_that_torch_did_not_make_take_turns():
+    """Which workspace a launch gets: its stream's last one, else one that has no memory yet, else the one that was not used for
+    the longest time.  (Every launch waits for the event of the one before it with the same workspace.)"""
+    from spork_b200 import api
+
+    pool = []
+    first = [api._whose_turn(pool, h) for h in (2, 64, 128, 192)]
+    assert len({id(e) for e in first}) == 4 and not any(e.clean or e.workspace for e in first)
+    for e in first:
+        e.workspace, e.clean = object(), True
+    assert api._whose_turn(pool, 2) is first[0] and api._whose_turn(pool, 64) is first[1]
+    assert api._whose_turn(pool, 256) is first[2] and first[2].handle == 256  # 128's was used longest ago
+    assert api._whose_turn(pool, 128) is first[3] and api._whose_turn(pool, 2) is first[0]
+    assert len(pool) == 4 and all(e.clean for e in pool)
+
+
 def test_wrappers_refuse_shapes_types_and_host_tensors(sp):
     import torch
 

@@ -617,6 +617,72 @@ def test_captured_graphs_follow_the_lengths(sp, cuda):
             assert torch.equal(w, o)
 
 
+def test_streams_that_torch_did_not_make(sp, cuda):
+    """The per-thread default stream, one handle for a stream of each thread, and streams that come and go under one handle:
+    no workspace is kept by such a handle, and launches that have one in common follow one another."""
+    import ctypes
+    import threading
+
+    import torch
+
+    from spork_b200 import api
+
+    cases = [Paged(cuda, [4000, 17, 800], 8, 2, 128, 16, torch.bfloat16, seed=s) for s in (1, 2, 3)]
+    want = [c.run(sp)[0] for c in cases]
+    kept = dict(api._workspaces)
+    outs = [[torch.empty_like(w) for _ in range(40)] for w in want]
+    torch.cuda.synchronize()
+    failed = []
+
+    def decode(i):
+        try:
+            c, s = cases[i], torch.cuda.ExternalStream(2, device=cuda)  # cudaStreamPerThread
+            for o in outs[i]:
+                sp.attn_paged(c.q, c.kc, c.vc, c.table, c.len, o, stream=s)
+            s.synchronize()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=decode, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    sp.status()
+    for w, os in zip(want, outs):
+        assert all(torch.equal(o, w) for o in os)
+
+    cudart = torch.cuda.cudart()
+    again = []
+    for i in range(12):  # more than there are workspaces; each is destroyed while its launch may still be under way
+        c, handle = cases[i % 3], ctypes.c_uint64()
+        assert int(cudart.cudaStreamCreate(ctypes.addressof(handle))) == 0
+        s = torch.cuda.ExternalStream(handle.value, device=cuda)
+        o = torch.empty_like(want[0])
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            sp.attn_paged(c.q, c.kc, c.vc, c.table, c.len, o)
+        assert int(cudart.cudaStreamDestroy(handle.value)) == 0
+        again.append(o)
+    torch.cuda.synchronize()
+    sp.status()
+    assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(again))
+    assert api._workspaces == kept and 1 <= len(api._lent[0]) <= 4
+
+    # after a launch that was given up the counters are cleared before the next use
+    for entry in api._lent[0]:
+        entry.workspace[:65536] = 1
+    assert sp.lib().spork_selftest_bounded_wait(1000, torch.cuda.current_stream().cuda_stream) == 0
+    with pytest.raises(sp.SporkError):
+        sp.status()
+    for o in outs[0]:
+        o.fill_(9.0)
+    torch.cuda.synchronize()
+    decode(0)
+    assert not failed and all(torch.equal(o, want[0]) for o in outs[0])
+
+
 def test_after_a_wait_that_ran_out(sp, cuda):
     """A launch that was given up may leave its workspace's counters as they were: once status() has said so, no kept
     workspace is used again, and the next calls of every stream are right."""
