@@ -801,3 +801,84 @@ def test_prompts_and_decoding_together(sp, cuda, dtype, graph):
             assert ((o[r].double() - whole.double()).abs() <= 2 * tol + weighted * 2 * (half + 1e-4)).all()
     sp.status()
     assert lengths.tolist() == [p + steps for p in prompts]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("graph", [False, True])
+def test_projection_store_and_attention_behind_one_another(sp, cuda, dtype, graph):
+    """The fp32 result of matmul_sm100 straight into the cache and the attention, step after step with nothing in between and
+    one buffer for the projection of all steps: each launch may begin before the one in front of it has ended, and waits
+    for it before it touches memory.  The outputs are those of steps that are waited for, bit for bit, and these are the
+    definition's."""
+    import torch
+
+    dtype = getattr(torch, dtype)
+    n, heads, kv_heads, dim, page, steps, width = 6, 8, 2, 64, 16, 40, 512
+    g = torch.Generator(device=cuda).manual_seed(3)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    x = torch.randn((steps, n, width), generator=g, device=cuda).half()
+    w = torch.randn(((heads + 2 * kv_heads) * dim, width), generator=g, device=cuda).mul_(width ** -0.5).half()
+    blocks = -(-steps // page)
+    free = torch.randperm(n * blocks, generator=g, device=cuda).to(torch.int32)
+    qkv = torch.empty((n, w.shape[0]), dtype=torch.float32, device=cuda)
+    q, k, v = (t.unflatten(1, (-1, dim)) for t in qkv.split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+    kc, vc = (torch.empty((n * blocks, kv_heads, page, dim), dtype=dtype, device=cuda) for _ in range(2))
+    table = torch.empty((n, blocks), **i32)
+    zeros, ones, none = torch.zeros(n, **i32), torch.ones(n, **i32), torch.zeros(1, **i32)
+
+    def decode(between):
+        lengths, used, outs = zeros, none, []
+        for i in range(steps):
+            sp.matmul_sm100(x[i], w, qkv, split_k=1)
+            slots, _, lengths, info = sp.paged_tables(lengths, ones, table, free, used, page_size=page, max_tokens=n)
+            sp.paged_store(k, v, kc, vc, slots)
+            outs.append(sp.attn_paged(q, kc, vc, table, lengths))
+            used = info[:1]
+            between()
+        return outs
+
+    def clear():
+        qkv.fill_(math.nan)
+        kc.fill_(math.nan)
+        vc.fill_(math.nan)
+        table.fill_(-1)
+        torch.cuda.synchronize()
+
+    projections = []
+
+    def keep():
+        torch.cuda.synchronize()
+        projections.append(qkv.clone())
+
+    clear()
+    want = decode(keep)
+    torch.cuda.synchronize()
+    sp.status()
+    for r in (0, n - 1):
+        for i in (0, 15, 16, steps - 1):
+            qs, ks, vs = torch.stack(projections[:i + 1])[:, r].split([heads * dim, kv_heads * dim, kv_heads * dim], 1)
+            keys, values = (t.unflatten(1, (kv_heads, dim)).transpose(0, 1).to(dtype) for t in (ks, vs))
+            query = qs[i].unflatten(0, (heads, dim))
+            ref, _, weighted, size = paged_plain.attention(query, keys, values, dim ** -0.5)
+            tol, _ = paged_plain.tolerances_of_fp32_queries(dtype, query, keys, dim ** -0.5, ref, weighted, size)
+            assert ((want[i][r].double() - ref).abs() <= tol).all(), (r, i)
+    # and the projection itself: 16-bit factors, exact products, sums of `width` of them in 32 bits
+    exact = x[steps - 1].double() @ w.double().t()
+    assert ((projections[-1].double() - exact).abs() <= width * 2.0 ** -23 * (x[steps - 1].double().abs() @ w.double().abs().t())).all()
+    if graph:
+        clear()
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            outs = decode(lambda: None)
+    for _ in range(3):
+        clear()
+        if graph:
+            for o in outs:
+                o.fill_(9.0)
+            captured.replay()
+            got = outs
+        else:
+            got = decode(lambda: None)
+        torch.cuda.synchronize()
+        sp.status()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
