@@ -1,13 +1,16 @@
 // Attention of one new token per request over a paged key-value cache, for sm_100a:
 //   o[r][h] = softmax(scale q[r][h] K^T) V over the keys that request r holds, key head h / (heads / kv_heads).
 //
-// Every key and value is read once and used by the few query heads that share it, so the kernel is bound by HBM; the
-// products are small.  Work is cut along the cache: units of 64 keys (128 with a head dimension of 64: 32 KB of keys and
-// values) of one (request, key head), all units in one list, request by request, and each block of the grid takes an
-// equal run of that list, whatever the lengths (they are known on the device only).  A block joins what it computes of
-// one (request, key head) and writes the result if it has all of it.  Otherwise it leaves a partial result (running
-// maximum, sum, unnormalised output) in the workspace and counts itself in; the block that comes last joins the parts,
-// in the order of the keys.  So one launch does, and what is added to what does not depend on who was last.
+// Every key and value is read once for up to 32 query heads that share it, and once more for every further 32.  With up
+// to 16 of them the products are small and the kernel is bound by HBM; from 17 on it is bound by the products, as every
+// instruction takes 8 heads (48 requests of 700..5003 keys, 2 key heads of 64: 20.3 us with 16 heads to one, 29 with
+// 32, 43 with 64, 75 with 128, of 10.4 to 11.5 that the bytes take).  Work is cut along the cache: units of 64 keys (128
+// with a head dimension of 64: 32 KB of keys and values) of one (request, key head), all units in one list, request by
+// request, and each block of the grid takes an equal run of that list, whatever the lengths (they are known on the
+// device only).  A block joins what it computes of one (request, key head) and writes the result if it has all of it.
+// Otherwise it leaves a partial result (running maximum, sum, unnormalised output) in the workspace and counts itself
+// in; the block that comes last joins the parts, in the order of the keys.  So one launch does, and what is added to
+// what does not depend on who was last.
 //
 // One warp copies the pages with TMA: the cache is a 5-dimensional tensor (64 elements, page rows, halves of the head
 // dimension, heads, pages) with the strides that it has, so any order in memory is one tensor map; a box is a page's
@@ -16,22 +19,24 @@
 //
 // Four warps compute, each on keys of its own, with mma.m16n8k16.  Up to 8 query heads are rows 0-7 of the 16-row
 // operand, and rows 8-15 hold what rounding to 16 bits left over: of q, if it is fp32, and of the softmax weights.  So
-// both products are taken with about 22 (fp16) or 16 (bf16) bits of q and of the weights at no cost: the rows would have
-// been empty, and the weights' rounding, the largest error of the usual scheme, is gone.  (Rows of fp32 queries are brought
-// into the 16-bit type's range by a power of two first.)  (tcgen05 would want 64 or 128
-// rows and a trip through tensor memory for every unit; the warp instruction's rate is several times what the loads can
-// feed.)  With 9 or more query heads to a key head the warps form 2 or 4 groups that share the unit, 8 heads each.
-// Each warp runs its own online softmax.  Its maximum follows the scores lazily: only when one has grown by more than
-// 2^8 over it are the row's lanes asked and the sums rescaled, so most units need no exchange between lanes at all.  The
-// warps of a group are joined once per (request, key head): each gets the others' sums for its share of the columns, and
-// writes that (or leaves it in the workspace, and joins that share of the parts).
+// both products are taken with about 22 (fp16) or 16 (bf16) bits of q and of the weights at no cost: the rows would
+// have been empty, and the weights' rounding, the largest error of the usual scheme, is gone.  (Rows of fp32 queries are
+// brought into the 16-bit type's range by a power of two first.)  (tcgen05 would want 64 or 128 rows and a trip through
+// tensor memory for every unit; up to 16 heads to one the warp instruction's rate is several times what the loads feed.)
+// With 9 or more query heads to a key head the warps form 2 or 4 groups that share the unit, 8 heads each.  Each warp
+// runs its own online softmax.  Its maximum follows the scores lazily: only when one has grown by more than 2^8 over it are the row's
+// lanes asked and the sums rescaled, so most units need no exchange between lanes at all.  The warps of a group are
+// joined once per (request, key head): each gets the others' sums for its share of the columns, and writes that (or
+// leaves it in the workspace, and joins that share of the parts).
 //
-// Measured (us a launch, in a stream of them; the share of the measured copy rate): 64 requests of 4096..8192 keys, 64 query
-// and 8 key heads of 128, bf16, 1.68 GB: 246..248 (104 %); 16 of 4096 keys, 16 heads of 128, 537 MB: 85..87 (94..96 %); one of 131072
-// keys, 32 / 8 heads: 86 (95 %); 23 of 1..6001 keys, 40 / 8 heads, fp32 q: 47 (82 %).  Of a short launch's time about 1.5 us
-// pass until a block knows its run (one trip to memory and a scan), 2 until its first keys are there, and 1.5 to 2.5 in the
-// joining of parts.  ncu (16 requests of the first shape): no local memory, mma.sync
-// at 17 % of its peak rate; of 11.5 warps between two instructions 5.9 wait for memory and 2.5 for a fixed latency.
+// Measured (us a launch, in a stream of them; the share of the measured copy rate): 64 requests of 4096..8192 keys, 64
+// query and 8 key heads of 128, bf16, 1.68 GB: 245..254 (101..105 %); 16 of 4096 keys, 16 heads of 128, 537 MB:
+// 85..88 (93..96 %); one of 131072 keys, 32 / 8 heads: 85..88 (93..96 %); 23 of 1..6001 keys, 40 / 8 heads, fp32 q: 46..48 (80..83 %);
+// 256 of 8..64 keys, 64 / 8 heads of 128, where each block has 6 or 7 short (request, key head)s one behind the other:
+// 18.5 (39 %).  Of a short launch's time about 1.5 us pass until a block knows its run (one trip to memory and a scan),
+// 2 until its first keys are there, and 1.5 to 2.5 in the joining of parts.  ncu (16 requests of the first shape, 8
+// heads to one): no local memory, mma.sync at 17 % of its peak rate; of 11.5 warps between two instructions 5.9 wait
+// for memory and 2.5 for a fixed latency.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -573,7 +578,8 @@ __device__ __forceinline__ uint32_t place_of(int first, int first_slot, int i)
 // A warp counts its share of this block's part in, which it has written.  The last of every kFan joins these in order and
 // leaves the result where the first of them was, and so on; the last of all writes the row of the output (o null: there is
 // none).  (The main loop bears no spills for this: with 200 bytes of them to a thread the kernel took up to 1.4 times as
-// long, since little of L1 is left beside the stages.)
+// long, since little of L1 is left beside the stages.  ptxas reports none, but for 20 bytes stored and 24 loaded where 9 to 16
+// heads of 128 with 16-bit queries share a key head; where those are was not looked at.)
 template <typename T, int kShare>
 __device__ __forceinline__ void join_parts(uint32_t* arrived, float2* part_ml, float* part_o, int first, int parts,
                                            int first_slot, T* o, float* lse)
@@ -1054,7 +1060,8 @@ static EncodeTiledFn encode_tiled_fn()
 
 // Query heads of a key head are taken 8, 16 or 32 at a time (groups of warps that share the keys in shared memory): the
 // fewest that hold them all, as empty rows cost a group's time.  us with 8 / 16 / 32 for 64 requests of 4096..8192 keys, 8 to
-// one, D = 128: 248 / 255 / 331; the same with 16 to one, with 16 / 32: 248 / 346.
+// one, D = 128: 245 / 252 / 333; the same with 16 to one, with 16 / 32: 246 / 345.  For 48 requests of 700..5003 keys, D = 64:
+// 4 and 8 to one 19.5 / 21.6 / 29.1 and 18.3 / 20.0 / 27.1, 16 to one 20.3 / 27.2.
 static int groups_of(int group) { return group <= kHeads ? 1 : group <= 2 * kHeads ? 2 : 4; }
 static int blocks_of(int sm_count) { return kBlocksPerSm * sm_count; }
 

@@ -24,8 +24,9 @@ using namespace spork::ptx;
 // requests for itself, keeps them in shared memory, and then fills its share of the slot map and of the new table
 // entries, finding the request of a token or page by bisection: one launch, and blocks that do not wait for one another.
 // A decoding step is bound by the latency of one dependent chain (lengths, sums, page, slot); a queue of prompts by
-// its bisections and the sums.  Measured: 256 decoding requests 4.5 us a launch, 2048 prompts of 1024 tokens 10.9 us, which
-// is 0.79 TB/s and an eighth of what writing the slot map alone would allow.
+// its slot map and the sums.  Measured: 256 decoding requests 4.5 us a launch; 2048 prompts of 1..1024 tokens (1.04 M in all)
+// 10.6 to 11.0 us, 0.8 TB/s of what it has to read and write; 2048 of 1..128 tokens, the same sums with an eighth of the map,
+// 6.3 us; 1024 of 1..1024 tokens 7.4 us.
 
 constexpr int kTableThreads = 1024;
 constexpr uint32_t kMost = 0x7FFFFFFF;
@@ -354,7 +355,7 @@ static int launch_tables(const spork_paged_tables_args& a, DeviceState& dev, cud
 {
     // One token to a thread while a block on every SM holds them all: the page numbers of decoding requests are then
     // looked up side by side.  Beyond that four, which mostly are one request's and in one page.  us with one / with four:
-    // 256 decoding requests 4.5 / 6.1, 4096 decoding requests 8.7 / 11.5, 2048 prompts of 1024 tokens 12.9 / 10.9.
+    // 256 decoding requests 4.5 / 6.1, 4096 decoding requests 8.7 / 11.5, 2048 prompts of 1..1024 tokens 12.9 / 10.9.
     const int64_t most = dev.sm_count, wanted = (a.max_tokens + kTableThreads - 1) / kTableThreads;
     if (wanted <= most) {
         return launch_tables<1>(a, dev, (unsigned)(wanted < 1 ? 1 : wanted), stream);
