@@ -408,7 +408,8 @@ int spork_paged_sm100_tables(const spork_paged_tables_args* args, void* stream);
  * cache's type if it is of another one.  src_type is the cache's type or
  * SPORK_TYPE_F32 (what the GEMMs write).  A slot outside the cache (-1, say)
  * writes nothing.  Slots within the cache must differ: of two tokens with the same
- * one, either's values may remain, piece by piece.  A token's keys and values together
+ * one, either's values may remain, piece by piece.  k and v must not overlap the
+ * cache, nor its halves one another.  A token's keys and values together
  * come to fewer than about 2^31 pieces (SPORK_ERR_TOO_LARGE): of 8 elements where
  * pointers, head_dim and strides allow 16 bytes of the cache at a time, else of one. */
 typedef struct spork_paged_store_args {
@@ -429,7 +430,8 @@ int spork_paged_sm100_store(const spork_paged_store_args* args, void* stream);
  *   request r, of key head h / (heads / kv_heads)
  * q [requests][heads][head_dim] at the given strides (elements), of the cache's type
  * or fp32; o contiguous, of the cache's type; lse (may be null) [requests][heads]: the
- * logarithm of the sum of the exponentials, fp32.  A request with no keys gets zeros
+ * logarithm of the sum of the exponentials, fp32.  o, lse and the workspace must not
+ * overlap anything else, nor the table's rows one another.  A request with no keys gets zeros
  * and -infinity; one with a negative length, a length beyond its table row or a page
  * outside the cache among those it needs gets NaN, and nothing outside the cache is
  * read.  Entries of a table row behind the last page that is needed, and rows of that

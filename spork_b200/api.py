@@ -717,7 +717,7 @@ def paged_store(k, v, k_cache, v_cache, slots, stream=None):
     the cache's type or float32 (what the GEMMs write; rounded to nearest even).  ``k_cache`` and ``v_cache`` are (num_pages,
     kv_heads, page_size, head_dim) float16 or bfloat16, the first three dimensions in any order in memory.  ``slots`` (T,)
     int64 is page * page_size + row, as paged_tables gives it; a slot outside the cache (-1) writes nothing, and slots
-    inside it must differ from each other."""
+    inside it must differ from each other.  ``k`` and ``v`` must not overlap the cache, nor its halves each other."""
     torch = _T or _bind_torch()
     shape, code, ks, vs = _pages(k_cache, v_cache)
     pages, kv_heads, page, dim = shape
@@ -808,7 +808,7 @@ def attn_paged(q, k_cache, v_cache, block_table, lengths, o=None, *, lse=None, s
     One new token per request: ``q`` is (R, heads, head_dim) of the cache's type or float32, with the last dimension
     contiguous; ``heads`` is a multiple of kv_heads, and query head h reads key head h // (heads // kv_heads).  ``k_cache``
     and ``v_cache`` are (num_pages, kv_heads, page_size, head_dim), the first three dimensions in any order in memory;
-    ``block_table`` (R, max_blocks) and ``lengths`` (R,) are int32.  ``o`` (contiguous) has the cache's type.  ``lse``, if
+    ``block_table`` (R, max_blocks), whose rows must not overlap, and ``lengths`` (R,) are int32.  ``o`` (contiguous) has the cache's type.  ``lse``, if
     given, is (R, heads) float32 and receives the logarithm of each softmax's sum.  A request of length 0 gets zeros (lse
     -inf); one with a length outside its table row or a page outside the cache gets NaN.  No gradient goes through it.
     Softmax weights, and ``q`` where it is float32, are taken as two parts of the cache's type each: 22 bits with float16, 16
